@@ -70,6 +70,10 @@ typedef enum PdnnActivation { PDNN_ACT_NONE = -1, PDNN_ACT_RELU = 0, PDNN_ACT_TA
 /* The remaining sycldnn::pointwise operators (Exp, Log, Floor, Sqrt): accepted by pdnn_pointwise
  * and, except Floor, pdnn_pointwise_grad, which take either enum; not valid as a fused activation. */
 typedef enum PdnnPointwiseOp { PDNN_PW_EXP = 3, PDNN_PW_LOG = 4, PDNN_PW_FLOOR = 5, PDNN_PW_SQRT = 6 } PdnnPointwiseOp;
+/* Activations without a counterpart in the reference, which the fused matrix product and the residual norm take beside
+ * those of PdnnActivation: x * Phi(x) with the normal distribution's function Phi (the erf form), x * sigmoid(x) and
+ * sigmoid(x).  The other calls refuse them. */
+typedef enum PdnnBlockActivation { PDNN_ACT_GELU = 7, PDNN_ACT_SILU = 8, PDNN_ACT_SIGMOID = 9 } PdnnBlockActivation;
 
 /* Field-for-field mirror of sycldnn::conv2d::Conv2DParams (include/portdnn/conv2d/params.h:32-112).
  * input_format: 0 NHWC, 1 NCHW (include/portdnn/data_format.h:31-43); filter_format: 0 HWCF, 1 FCHW,
@@ -312,6 +316,115 @@ int pdnn_transpose(int elem_bytes, const void* input, void* output, const int* d
  * out[b] = beta*out[b] + op(lhs[b]) * op(rhs[b]), row-major, strided batches. */
 int pdnn_matmul(int dtype, int transpose_lhs, int transpose_rhs, const void* lhs, const void* rhs, void* output,
                 int batches, int m, int k, int n, float beta, void* stream);
+
+/* ---- around the matrix products of a network's blocks (no counterpart in the reference) --------------------
+ * Pitches are the distance between two rows in elements, 0 standing for dense rows; rows may be part of wider ones, whose
+ * other columns are neither read nor written.  No alignment is asked for: operands that the tensor cores cannot read in
+ * place (16-bit rows off a 16-byte boundary, or whose pitch is no multiple of 16 bytes) are copied to scratch from the
+ * stream-ordered allocator first.  Sums are held in 32 bits; a result is rounded once.  The order in which the products of
+ * an output are added depends on the sizes.  Results have the same bits in every call of the same sizes. */
+
+/* lhs [m][k], rhs [k][n] (transpose_rhs: [n][k]), output [m][n].  m may be 0. */
+typedef struct PdnnMatmulParams {
+  int m, k, n, transpose_rhs;
+  long long lhs_pitch, rhs_pitch, output_pitch;
+} PdnnMatmulParams;
+
+/* z = lhs * rhs + bias;  output = residual + scale * activation(z).  pre_activation: z, for the gradient.  Null tensors
+ * are left out.  The residual may be the output's own buffer (with the same pitch). */
+typedef struct PdnnMatmulEpilogue {
+  const void* bias; /* [n] */
+  int activation;   /* PdnnActivation or PdnnBlockActivation */
+  float scale;
+  const void* residual; /* [m][n] */
+  long long residual_pitch;
+  void* pre_activation; /* [m][n] */
+  long long pre_activation_pitch;
+} PdnnMatmulEpilogue;
+
+/* epilogue NULL: the plain product. */
+int pdnn_matmul_fused(int dtype, const void* lhs, const void* rhs, void* output, const PdnnMatmulParams* params,
+                      const PdnnMatmulEpilogue* epilogue, void* stream);
+
+/* The gradients of pdnn_matmul_fused: with dy = output_grad ([m][n], pitch params->output_pitch)
+ *   dz = scale * dy * activation'(pre_activation)
+ *   lhs_grad  = dz * rhs^T, times input_activation'(input_pre_activation) where that is given: the gradient with respect to
+ *               what the layer before had put through its activation (lhs is its result)
+ *   rhs_grad  = lhs^T * dz, in rhs' own layout
+ *   bias_grad = sum of dz over its rows
+ * Null results are left out; the residual's gradient is dy itself.  For 16-bit tensors dz is rounded to their type, which is
+ * what the tensor cores multiply (bias_grad sums the values ahead of that rounding, unless dz is dy itself).  lhs_grad may
+ * not be one of the inputs' buffers.  m == 0 leaves rhs_grad and bias_grad zero. */
+typedef struct PdnnMatmulGradient {
+  int activation; /* PDNN_ACT_NONE: pre_activation is not read */
+  float scale;
+  const void* pre_activation; /* [m][n] */
+  long long pre_activation_pitch;
+  int input_activation;
+  const void* input_pre_activation; /* [m][k] */
+  long long input_pre_activation_pitch;
+  void *lhs_grad, *rhs_grad, *bias_grad;
+  long long lhs_grad_pitch, rhs_grad_pitch;
+} PdnnMatmulGradient;
+int pdnn_matmul_fused_gradient(int dtype, const void* output_grad, const void* lhs, const void* rhs,
+                               const PdnnMatmulParams* params, const PdnnMatmulGradient* gradient, void* stream);
+
+/* The norms around a block, its gate and its residual sum:
+ *   n = post_norm(branch);  sum = residual + scale * gate_activation(gate) * n;  output = pre_norm(sum)
+ * post_norm normalises what the block has put out, pre_norm what the next block reads.  A norm takes each row's mean
+ * square (PDNN_NORM_RMS), or mean and variance (PDNN_NORM_LAYER), over its channels.  Tensors are dense [rows][channels];
+ * gammas and betas have `channels` entries (NULL: ones and zeros); the gate is [gate_groups][channels], and each of its rows
+ * serves rows / gate_groups consecutive rows (1: all rows; rows: each row its own).  rows may be 0. */
+typedef enum PdnnNorm { PDNN_NORM_NONE = 0, PDNN_NORM_RMS = 1, PDNN_NORM_LAYER = 2 } PdnnNorm;
+typedef struct PdnnResidualNormParams {
+  int rows, channels, post_norm, pre_norm;
+  int gate_groups, gate_activation; /* 0 groups: no gate */
+  float scale, epsilon;
+} PdnnResidualNormParams;
+
+/* sum or output may be NULL, and residual (zeros).  sum may be the residual's own buffer and output the branch's.
+ * statistics ([4][rows] floats; may be NULL): mean and reciprocal deviation that post_norm took, and those of pre_norm (0 and 1
+ * where a norm takes none); the gradient reads them.  output and statistics are of the sum in 32 bits. */
+typedef struct PdnnResidualNormTensors {
+  const void *branch, *residual, *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
+  void *sum, *output;
+  float* statistics;
+} PdnnResidualNormTensors;
+int pdnn_residual_norm(int dtype, const PdnnResidualNormParams* params, const PdnnResidualNormTensors* tensors, void* stream);
+
+/* Its gradients.  Of `tensors` branch, sum, statistics, the gammas, post_beta and the gate are read.  sum_grad is what
+ * arrives at the sum by the residual stream (NULL: nothing), output_grad what arrives at the output.  Null results are left
+ * out.  residual_grad may be sum_grad's buffer and branch_grad output_grad's.  Sums over rows are taken in a fixed order. */
+typedef struct PdnnResidualNormGradients {
+  const void *sum_grad, *output_grad;
+  void *branch_grad, *residual_grad, *post_gamma_grad, *post_beta_grad, *gate_grad, *pre_gamma_grad, *pre_beta_grad;
+} PdnnResidualNormGradients;
+int pdnn_residual_norm_gradient(int dtype, const PdnnResidualNormParams* params, const PdnnResidualNormTensors* tensors,
+                                const PdnnResidualNormGradients* gradients, void* stream);
+
+/* Clipped policy loss of sampled tokens, with an estimate of the divergence from a reference policy, and its gradient:
+ *   logp  = logits[target] / temperature - log sum exp(logits / temperature)
+ *   ratio = exp(logp - old_logp)                            (old_logp NULL: logp itself, so that ratio is 1)
+ *   loss  = weight * (-min(ratio * advantage, clip(ratio, 1 - clip_low, 1 + clip_high) * advantage)
+ *                     + kl * (exp(ref_logp - logp) - (ref_logp - logp) - 1))            (ref_logp NULL: without the last term)
+ *   grad  = grad_scale * d loss / d logits
+ * logits: `rows` rows of `vocab` entries; targets: whole numbers of target_bytes (4 or 8) bytes; advantages, old_logp, ref_logp,
+ * weights (NULL: ones): floats, one to a row.  loss: one float, the sum of token_loss; token_loss, logp: [rows] floats.
+ * grad (NULL: forward only) has the logits' type and may be their own buffer, with the same pitch.
+ * A row counts for nothing - loss, logp and gradient 0, whatever its logits hold - where its weight is 0 or its target
+ * lies outside [0, vocab); so does one whose logits are all minus infinity.  rows may be 0. */
+typedef struct PdnnPolicyLossParams {
+  int rows, vocab, target_bytes;
+  float clip_low, clip_high, kl, temperature, grad_scale;
+  long long logits_pitch, grad_pitch;
+} PdnnPolicyLossParams;
+typedef struct PdnnPolicyLossTensors {
+  const void *logits, *targets;
+  const float *advantages, *old_logp, *ref_logp, *weights;
+  float *loss, *token_loss, *logp;
+  void* grad;
+} PdnnPolicyLossTensors;
+int pdnn_policy_loss(int dtype, const PdnnPolicyLossParams* params, const PdnnPolicyLossTensors* tensors, void* stream);
 
 /* The collective of the batch-sharded path; no counterpart in the reference, which is single-device.
  * Each rank's filter-backprop pass leaves fp32 gradients for its shard of the batch in one contiguous

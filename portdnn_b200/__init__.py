@@ -12,13 +12,15 @@ from .api import (  # noqa: F401
     F32, F16, BF16,
     ALGO_DIRECT, ALGO_TILED, ALGO_IM2COL, ALGO_WINOGRAD, ALGO_WINOGRAD_LARGE, ALGO_MATMUL,
     POOL_MAX, POOL_MAX_WITH_NAN, POOL_AVERAGE,
-    ACT_NONE, ACT_RELU, ACT_TANH, ACT_RELU6,
+    ACT_NONE, ACT_RELU, ACT_TANH, ACT_RELU6, ACT_GELU, ACT_SILU, ACT_SIGMOID, NORM_NONE, NORM_RMS, NORM_LAYER,
     PW_EXP, PW_LOG, PW_FLOOR, PW_SQRT, BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV,
     StatusCode, PortDNNError,
     Conv2DParams, DepthwiseConv2DParams, PoolingParams, SoftmaxParams, BatchNormParams,
+    ResidualNormParams,
     conv_params, depthwise_params, pool_params, calculate_padding,
     conv2d, conv2d_workspace_size, conv2d_validate, depthwise_conv2d, pooling, pooling_max_grad,
     pointwise, pointwise_grad, bias_add, binaryop, scale_blend, matmul, transpose,
     softmax, batchnorm_params, batchnorm_forward, batchnorm_gradient,
+    matmul_fused, matmul_fused_grad, residual_norm_params, residual_norm, residual_norm_grad, policy_loss,
     device_error_record, last_gemm_kernel, launch_count, lib, library_path,
 )

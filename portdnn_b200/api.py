@@ -22,6 +22,8 @@ F32, F16, BF16 = 0, 1, 2
 ALGO_DIRECT, ALGO_TILED, ALGO_IM2COL, ALGO_WINOGRAD, ALGO_WINOGRAD_LARGE, ALGO_MATMUL = 1, 2, 3, 4, 5, 6
 POOL_MAX, POOL_MAX_WITH_NAN, POOL_AVERAGE = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_TANH, ACT_RELU6 = -1, 0, 1, 2
+ACT_GELU, ACT_SILU, ACT_SIGMOID = 7, 8, 9  # the fused matrix product and the residual norm only
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV = 0, 1, 2, 3
 PW_EXP, PW_LOG, PW_FLOOR, PW_SQRT = 3, 4, 5, 6  # the other sycldnn::pointwise operators (pointwise() only)
 
@@ -74,6 +76,12 @@ class BatchNormParams(ctypes.Structure):
     """sycldnn::batchnorm::BatchNormParams, include/portdnn/batchnorm/params.h:32-72."""
     _fields_ = _ints("batch", "rows", "cols", "channels", "is_training") + \
         [("epsilon", ctypes.c_float), ("momentum", ctypes.c_float), ("input_format", ctypes.c_int)]
+
+
+class ResidualNormParams(ctypes.Structure):
+    """PdnnResidualNormParams."""
+    _fields_ = _ints("rows", "channels", "post_norm", "pre_norm", "gate_groups", "gate_activation") + \
+        [("scale", ctypes.c_float), ("epsilon", ctypes.c_float)]
 
 
 def library_path():
@@ -334,6 +342,65 @@ def batchnorm_gradient(inp, gradient, gamma, params, pop_mean=None, pop_variance
     """batchnorm::launch<T, Backend, Gradient> (include/portdnn/batchnorm/launch.h:332-444)
     -> (input gradient, beta gradient, gamma gradient)."""
     return (_F or _front()).batchnorm_gradient(inp, gradient, gamma, params, pop_mean, pop_variance, out)
+
+
+def matmul_fused(lhs, rhs, transpose_rhs=False, bias=None, activation=ACT_NONE, residual=None, scale=1.0,
+                 pre_activation=None, out=None):
+    """residual + scale * activation(lhs @ rhs + bias) in one call (pdnn_matmul_fused; no counterpart in the reference).
+    lhs [m, k], rhs [k, n] ([n, k] with transpose_rhs), bias [n], residual and the result [m, n], all of one type; rows may
+    lie any distance apart (slices of wider tensors).  pre_activation: a tensor that receives lhs @ rhs + bias, which the
+    gradient reads.  activation: ACT_RELU, ACT_TANH, ACT_RELU6, ACT_GELU, ACT_SILU, ACT_SIGMOID or ACT_NONE.  out may be the
+    residual.  Runs on the tensors' device, on its current stream."""
+    return (_F or _front()).matmul_fused(lhs, rhs, transpose_rhs, bias, activation, residual, scale, pre_activation, out)
+
+
+def matmul_fused_grad(grad, lhs, rhs, transpose_rhs=False, activation=ACT_NONE, pre_activation=None, scale=1.0,
+                      input_activation=ACT_NONE, input_pre_activation=None, want_lhs_grad=True, want_rhs_grad=True,
+                      want_bias_grad=True, lhs_grad=None, rhs_grad=None, bias_grad=None):
+    """Gradients of matmul_fused (pdnn_matmul_fused_gradient) -> (lhs_grad, rhs_grad, bias_grad), None for those not wanted;
+    the residual's is grad itself.  With dz = scale * grad * activation'(pre_activation): lhs_grad = dz @ rhs^T, rhs_grad =
+    lhs^T @ dz in rhs' own layout, bias_grad = sum of dz's rows.  input_activation and input_pre_activation: lhs is what that
+    activation made of that tensor, and lhs_grad is to be the gradient with respect to the latter."""
+    return (_F or _front()).matmul_fused_grad(grad, lhs, rhs, transpose_rhs, activation, pre_activation, scale,
+                                              input_activation, input_pre_activation, want_lhs_grad, want_rhs_grad,
+                                              want_bias_grad, lhs_grad, rhs_grad, bias_grad)
+
+
+def residual_norm_params(rows, channels, post_norm=NORM_RMS, pre_norm=NORM_RMS, gate_groups=0, gate_activation=ACT_NONE,
+                         scale=1.0, epsilon=1e-6):
+    return ResidualNormParams(rows, channels, post_norm, pre_norm, gate_groups, gate_activation, scale, epsilon)
+
+
+def residual_norm(branch, residual, params, post_gamma=None, post_beta=None, gate=None, pre_gamma=None, pre_beta=None,
+                  sum_out=None, out=None):
+    """The norms around a block with its gate and residual sum (pdnn_residual_norm; no counterpart in the reference):
+    sum = residual + scale * gate_activation(gate) * post_norm(branch), out = pre_norm(sum) -> (sum, out, statistics).
+    branch, residual (None: zeros), sum and out: dense [rows, channels]; gammas and betas [channels] (None: ones, zeros);
+    gate [gate_groups, channels], a row of it to rows / gate_groups rows.  sum_out may be the residual, out the branch."""
+    return (_F or _front()).residual_norm(branch, residual, params, post_gamma, post_beta, gate, pre_gamma, pre_beta, sum_out,
+                                          out)
+
+
+def residual_norm_grad(sum_grad, output_grad, branch, sum, statistics, params, post_gamma=None, post_beta=None, gate=None,
+                       pre_gamma=None, pre_beta=None, branch_grad=None, residual_grad=None):
+    """Gradients of residual_norm (pdnn_residual_norm_gradient) -> (branch_grad, residual_grad, post_gamma_grad,
+    post_beta_grad, gate_grad, pre_gamma_grad, pre_beta_grad), None for parameters that are None.  sum_grad (None: zeros) is
+    what arrives at the sum by the residual stream, output_grad what arrives at the normalised output; sum and statistics
+    are the forward call's.  branch_grad may be output_grad, residual_grad sum_grad."""
+    return (_F or _front()).residual_norm_grad(sum_grad, output_grad, branch, sum, statistics, params, post_gamma, post_beta,
+                                               gate, pre_gamma, pre_beta, branch_grad, residual_grad)
+
+
+def policy_loss(logits, targets, advantages, old_logp=None, ref_logp=None, weights=None, clip_low=0.2, clip_high=0.2, kl=0.0,
+                temperature=1.0, grad_scale=1.0, want_grad=True, grad=None):
+    """Clipped policy loss of sampled tokens with a KL term, and its gradient with respect to the logits, in one call
+    (pdnn_policy_loss; no counterpart in the reference) -> (loss, token_loss, logp, grad).  logits [rows, vocab], whose rows may
+    lie any distance apart (a vocabulary padded to a wider row); targets [rows] of 32 or 64 bits; advantages, old_logp (None:
+    the policy's own), ref_logp (None: no KL term) and weights (None: ones) [rows] in float32.  loss is the sum of token_loss.
+    A row whose weight is 0 or whose target lies outside the vocabulary counts for nothing and is not read.  grad may be
+    the logits."""
+    return (_F or _front()).policy_loss(logits, targets, advantages, old_logp, ref_logp, weights, clip_low, clip_high, kl,
+                                        temperature, grad_scale, want_grad, grad)
 
 
 def device_error_record(clear=True):

@@ -1,4 +1,5 @@
 // extern "C" entry points declared in include/portdnn_b200.h.
+#include "activation.cuh"
 #include "common.cuh"
 #include "padded_conv.cuh"
 #include "simt_gemm.cuh"
@@ -474,6 +475,89 @@ int pdnn_matmul(int dtype, int transpose_lhs, int transpose_rhs, const void* lhs
   if (tc_matmul_supported(dtype, tl, tr, lhs, rhs, output, batches, m, k, n))
     return tc_matmul(dtype, tl, tr, lhs, rhs, output, batches, m, k, n, beta, s);
   return simt_matmul(dtype, tl, tr, lhs, rhs, output, batches, m, k, n, beta, s);
+}
+
+namespace {
+// Sizes of a fused product, its pitches filled in, and whether it can run at all.
+int check_matmul_fused(const char* what, int dtype, PdnnMatmulParams& p) {
+  if (dtype < PDNN_F32 || dtype > PDNN_BF16) return fail(PDNN_INVALID_PARAMETER, "%s: unknown dtype %d", what, dtype);
+  if (p.m < 0 || p.k <= 0 || p.n <= 0) return fail(PDNN_INVALID_PARAMETER, "%s: sizes %d, %d, %d", what, p.m, p.k, p.n);
+  p.transpose_rhs = p.transpose_rhs != 0;
+  struct {
+    long long* pitch;
+    int row;
+  } const rows[3] = {{&p.lhs_pitch, p.k}, {&p.rhs_pitch, p.transpose_rhs ? p.k : p.n}, {&p.output_pitch, p.n}};
+  for (const auto& r : rows) {
+    if (*r.pitch == 0) *r.pitch = r.row;
+    if (*r.pitch < r.row) return fail(PDNN_INVALID_PARAMETER, "%s: a row's pitch is shorter than the row", what);
+  }
+  if (device_sm_count() <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
+  return PDNN_OK;
+}
+int fill_pitch(const char* what, const void* tensor, long long& pitch, int row) {
+  if (pitch == 0) pitch = row;
+  if (tensor != nullptr && pitch < row) return fail(PDNN_INVALID_PARAMETER, "%s: a row's pitch is shorter than the row", what);
+  return PDNN_OK;
+}
+}  // namespace
+
+int pdnn_matmul_fused(int dtype, const void* lhs, const void* rhs, void* output, const PdnnMatmulParams* params,
+                      const PdnnMatmulEpilogue* epilogue, void* stream) {
+  const char* what = "matmul_fused";
+  if (params == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null params", what);
+  PdnnMatmulParams p = *params;
+  PdnnMatmulEpilogue e = {};
+  e.activation = PDNN_ACT_NONE;
+  e.scale = 1.f;
+  if (epilogue != nullptr) e = *epilogue;
+  if (!known_activation(e.activation)) return fail(PDNN_INVALID_PARAMETER, "%s: unknown activation %d", what, e.activation);
+  int st = check_matmul_fused(what, dtype, p);
+  if (st == PDNN_OK) st = fill_pitch(what, e.residual, e.residual_pitch, p.n);
+  if (st == PDNN_OK) st = fill_pitch(what, e.pre_activation, e.pre_activation_pitch, p.n);
+  if (st != PDNN_OK || p.m == 0) return st;
+  if (lhs == nullptr || rhs == nullptr || output == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  return launch_matmul_fused(dtype, lhs, rhs, output, p, e, static_cast<cudaStream_t>(stream));
+}
+
+int pdnn_matmul_fused_gradient(int dtype, const void* output_grad, const void* lhs, const void* rhs,
+                               const PdnnMatmulParams* params, const PdnnMatmulGradient* gradient, void* stream) {
+  const char* what = "matmul_fused gradient";
+  if (params == nullptr || gradient == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null params", what);
+  PdnnMatmulParams p = *params;
+  PdnnMatmulGradient g = *gradient;
+  if (!known_activation(g.activation) || !known_activation(g.input_activation))
+    return fail(PDNN_INVALID_PARAMETER, "%s: unknown activation", what);
+  int st = check_matmul_fused(what, dtype, p);
+  if (st == PDNN_OK) st = fill_pitch(what, g.pre_activation, g.pre_activation_pitch, p.n);
+  if (st == PDNN_OK) st = fill_pitch(what, g.input_pre_activation, g.input_pre_activation_pitch, p.k);
+  if (st == PDNN_OK) st = fill_pitch(what, g.lhs_grad, g.lhs_grad_pitch, p.k);
+  if (st == PDNN_OK) st = fill_pitch(what, g.rhs_grad, g.rhs_grad_pitch, p.transpose_rhs ? p.k : p.n);
+  if (st != PDNN_OK) return st;
+  if (p.m > 0) {
+    if (output_grad == nullptr || (g.lhs_grad != nullptr && rhs == nullptr) || (g.rhs_grad != nullptr && lhs == nullptr))
+      return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+    if ((g.activation != PDNN_ACT_NONE && g.pre_activation == nullptr) ||
+        (g.input_activation != PDNN_ACT_NONE && g.lhs_grad != nullptr && g.input_pre_activation == nullptr))
+      return fail(PDNN_INVALID_PARAMETER, "%s: an activation's gradient needs what the activation was applied to", what);
+  }
+  return launch_matmul_fused_gradient(dtype, output_grad, lhs, rhs, p, g, static_cast<cudaStream_t>(stream));
+}
+
+int pdnn_residual_norm(int dtype, const PdnnResidualNormParams* params, const PdnnResidualNormTensors* tensors, void* stream) {
+  if (params == nullptr || tensors == nullptr) return fail(PDNN_INVALID_PARAMETER, "residual norm: null params");
+  return launch_residual_norm(dtype, *params, *tensors, static_cast<cudaStream_t>(stream));
+}
+
+int pdnn_residual_norm_gradient(int dtype, const PdnnResidualNormParams* params, const PdnnResidualNormTensors* tensors,
+                                const PdnnResidualNormGradients* gradients, void* stream) {
+  if (params == nullptr || tensors == nullptr || gradients == nullptr)
+    return fail(PDNN_INVALID_PARAMETER, "residual norm gradient: null params");
+  return launch_residual_norm_gradient(dtype, *params, *tensors, *gradients, static_cast<cudaStream_t>(stream));
+}
+
+int pdnn_policy_loss(int dtype, const PdnnPolicyLossParams* params, const PdnnPolicyLossTensors* tensors, void* stream) {
+  if (params == nullptr || tensors == nullptr) return fail(PDNN_INVALID_PARAMETER, "policy loss: null params");
+  return launch_policy_loss(dtype, *params, *tensors, static_cast<cudaStream_t>(stream));
 }
 
 int pdnn_device_error_record(unsigned words[4], int clear) {

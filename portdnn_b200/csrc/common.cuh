@@ -203,6 +203,20 @@ int launch_batchnorm_gradient(int dtype, const void* input, const void* gradient
                               const void* pop_mean, const void* pop_variance, void* beta_grad, void* gamma_grad,
                               void* output, const PdnnBatchNormParams& p, cudaStream_t s);
 
+// the norms around a block with its gate and residual sum (residual_norm.cu)
+int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnResidualNormTensors& t, cudaStream_t s);
+int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, const PdnnResidualNormTensors& t,
+                                  const PdnnResidualNormGradients& g, cudaStream_t s);
+
+// the clipped policy loss (policy_loss.cu)
+int launch_policy_loss(int dtype, const PdnnPolicyLossParams& p, const PdnnPolicyLossTensors& t, cudaStream_t s);
+
+// the matrix product with its epilogue, and its gradients (fused_matmul.cu); pitches are filled in and checked
+int launch_matmul_fused(int dtype, const void* lhs, const void* rhs, void* out, const PdnnMatmulParams& p,
+                        const PdnnMatmulEpilogue& e, cudaStream_t s);
+int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, const void* rhs, const PdnnMatmulParams& p,
+                                 const PdnnMatmulGradient& g, cudaStream_t s);
+
 // Winograd F(2x2,3x3) (winograd.cu): forward and input backprop of 3x3 stride-1 layers.
 bool winograd_applicable(int pass, int dtype, const PdnnConv2DParams& p);
 size_t winograd_workspace_elems(int pass, int dtype, const PdnnConv2DParams& p);

@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -436,6 +437,284 @@ PyObject* batchnorm_gradient(PyObject* const* a) {
   return triple(out, bg, gg);
 }
 
+// ---- the operators around a block's matrix products -----------------------------------------------------
+
+// A matrix argument: two dimensions, a row's elements next to each other, rows any distance apart.
+struct MatrixArg {
+  at::Tensor t;
+  int64_t rows = 0, cols = 0;
+  long long pitch = 0;
+};
+MatrixArg matrix(PyObject* o, const char* name) {
+  MatrixArg m;
+  m.t = tensor(o);
+  if (!m.t.defined()) return m;
+  if (!m.t.is_cuda() || m.t.dim() != 2) raise(PyExc_ValueError, "%s must be a CUDA tensor of two dimensions", name);
+  m.rows = m.t.size(0);
+  m.cols = m.t.size(1);
+  const bool one_row = m.rows <= 1;
+  if (m.t.numel() > 0 && ((m.cols > 1 && m.t.stride(1) != 1) || (!one_row && m.t.stride(0) < m.cols)))
+    raise(PyExc_ValueError, "the elements of %s's rows must be next to each other, and its rows must not overlap", name);
+  m.pitch = one_row || m.t.numel() == 0 ? m.cols : m.t.stride(0);
+  return m;
+}
+void require_shape(const MatrixArg& m, int64_t rows, int64_t cols, const at::Tensor& like, const char* name) {
+  if (!m.t.defined()) return;
+  if (m.rows != rows || m.cols != cols)
+    raise(PyExc_ValueError, "%s must be [%lld, %lld], not [%lld, %lld]", name, (long long)rows, (long long)cols, (long long)m.rows,
+          (long long)m.cols);
+  if (m.t.scalar_type() != like.scalar_type() || m.t.device() != like.device())
+    raise(PyExc_ValueError, "%s must have the other tensors' type and device", name);
+}
+// A vector, or another dense tensor, of so many elements.
+at::Tensor dense(PyObject* o, int64_t numel, const at::Tensor& like, at::ScalarType type, const char* name) {
+  const at::Tensor t = tensor(o);
+  if (!t.defined()) return t;
+  if (!t.is_cuda() || !t.is_contiguous()) raise(PyExc_ValueError, "tensors must be contiguous CUDA tensors");
+  if (t.numel() != numel) raise(PyExc_ValueError, "%s must have %lld elements, not %lld", name, (long long)numel, (long long)t.numel());
+  if (t.scalar_type() != type || t.device() != like.device())
+    raise(PyExc_ValueError, "%s must have the type %s and the other tensors' device", name, c10::toString(type));
+  return t;
+}
+at::Tensor dense(PyObject* o, int64_t numel, const at::Tensor& like, const char* name) {
+  return dense(o, numel, like, like.scalar_type(), name);
+}
+int extent(int64_t v) {
+  if (v > 0x7FFFFFFFll) raise(PyExc_ValueError, "an extent of %lld is too large", (long long)v);
+  return (int)v;
+}
+// The current device is the tensors' own while the library runs: a call with tensors of another device goes there, on that
+// device's current stream.
+struct OnDevice {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit OnDevice(const at::Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+MatrixArg new_matrix(int64_t rows, int64_t cols, const at::Tensor& like) {
+  MatrixArg m;
+  m.t = unlocked([&] { return at::empty({rows, cols}, like.options()); });
+  m.rows = rows;
+  m.cols = cols;
+  m.pitch = cols;
+  return m;
+}
+PyObject* wrap_or_none(const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
+template <size_t N>
+PyObject* tuple_of(const at::Tensor (&list)[N]) {
+  PyObject* t = PyTuple_New(N);
+  if (t == nullptr) throw PyFailure();
+  for (size_t i = 0; i < N; ++i) {
+    PyObject* o = wrap_or_none(list[i]);
+    if (o == nullptr) {
+      Py_DECREF(t);
+      throw PyFailure();
+    }
+    PyTuple_SET_ITEM(t, (Py_ssize_t)i, o);
+  }
+  return t;
+}
+
+PyObject* matmul_fused(PyObject* const* a) {
+  const MatrixArg lhs = matrix(a[0], "lhs"), rhs = matrix(a[1], "rhs");
+  if (!lhs.t.defined() || !rhs.t.defined()) raise(PyExc_ValueError, "lhs and rhs are needed");
+  const bool tr = truth(a[2]);
+  const int dtype = dtype_code(lhs.t);
+  const int64_t m = lhs.rows, k = lhs.cols, n = tr ? rhs.rows : rhs.cols;
+  require_shape(rhs, tr ? n : k, tr ? k : n, lhs.t, "rhs");
+  const at::Tensor bias = dense(a[3], n, lhs.t, "bias");
+  PdnnMatmulEpilogue e = {};
+  e.activation = (int)to_integer(a[4]);
+  const MatrixArg residual = matrix(a[5], "residual");
+  e.scale = (float)real(a[6]);
+  const MatrixArg pre = matrix(a[7], "pre_activation");
+  MatrixArg out = matrix(a[8], "out");
+  require_shape(residual, m, n, lhs.t, "residual");
+  require_shape(pre, m, n, lhs.t, "pre_activation");
+  require_shape(out, m, n, lhs.t, "out");
+  if (!out.t.defined()) out = new_matrix(m, n, lhs.t);
+  e.bias = ptr(bias);
+  e.residual = ptr(residual.t);
+  e.residual_pitch = residual.pitch;
+  e.pre_activation = ptr(pre.t);
+  e.pre_activation_pitch = pre.pitch;
+  const PdnnMatmulParams p = {extent(m), extent(k), extent(n), tr, lhs.pitch, rhs.pitch, out.pitch};
+  const OnDevice on(lhs.t);
+  call([&] { return pdnn_matmul_fused(dtype, ptr(lhs.t), ptr(rhs.t), ptr(out.t), &p, &e, on.stream); });
+  return THPVariable_Wrap(out.t);
+}
+
+PyObject* matmul_fused_grad(PyObject* const* a) {
+  const MatrixArg grad = matrix(a[0], "grad"), lhs = matrix(a[1], "lhs"), rhs = matrix(a[2], "rhs");
+  if (!grad.t.defined() || !lhs.t.defined() || !rhs.t.defined()) raise(PyExc_ValueError, "grad, lhs and rhs are needed");
+  const bool tr = truth(a[3]);
+  const int dtype = dtype_code(lhs.t);
+  const int64_t m = lhs.rows, k = lhs.cols, n = tr ? rhs.rows : rhs.cols;
+  require_shape(rhs, tr ? n : k, tr ? k : n, lhs.t, "rhs");
+  require_shape(grad, m, n, lhs.t, "grad");
+  PdnnMatmulGradient g = {};
+  g.activation = (int)to_integer(a[4]);
+  const MatrixArg pre = matrix(a[5], "pre_activation");
+  g.scale = (float)real(a[6]);
+  g.input_activation = (int)to_integer(a[7]);
+  const MatrixArg input_pre = matrix(a[8], "input_pre_activation");
+  const bool want[3] = {truth(a[9]), truth(a[10]), truth(a[11])};
+  MatrixArg dl = matrix(a[12], "lhs_grad"), dr = matrix(a[13], "rhs_grad");
+  at::Tensor db = dense(a[14], n, lhs.t, "bias_grad");
+  require_shape(pre, m, n, lhs.t, "pre_activation");
+  require_shape(input_pre, m, k, lhs.t, "input_pre_activation");
+  require_shape(dl, m, k, lhs.t, "lhs_grad");
+  require_shape(dr, rhs.rows, rhs.cols, lhs.t, "rhs_grad");
+  if (!dl.t.defined() && want[0]) dl = new_matrix(m, k, lhs.t);
+  if (!dr.t.defined() && want[1]) dr = new_matrix(rhs.rows, rhs.cols, lhs.t);
+  if (!db.defined() && want[2]) db = flat(n, lhs.t.options());
+  g.pre_activation = ptr(pre.t);
+  g.pre_activation_pitch = pre.pitch;
+  g.input_pre_activation = ptr(input_pre.t);
+  g.input_pre_activation_pitch = input_pre.pitch;
+  g.lhs_grad = ptr(dl.t);
+  g.lhs_grad_pitch = dl.pitch;
+  g.rhs_grad = ptr(dr.t);
+  g.rhs_grad_pitch = dr.pitch;
+  g.bias_grad = ptr(db);
+  const PdnnMatmulParams p = {extent(m), extent(k), extent(n), tr, lhs.pitch, rhs.pitch, grad.pitch};
+  const OnDevice on(lhs.t);
+  call([&] { return pdnn_matmul_fused_gradient(dtype, ptr(grad.t), ptr(lhs.t), ptr(rhs.t), &p, &g, on.stream); });
+  return tuple_of({dl.t, dr.t, db});
+}
+
+// Tensors of the residual norm that both directions read.
+struct NormTensors {
+  PdnnResidualNormParams p;
+  int64_t numel;
+  at::Tensor branch, post_gamma, post_beta, gate, pre_gamma, pre_beta;
+  NormTensors(PyObject* b, PyObject* params_, PyObject* const* vectors) : p(params<PdnnResidualNormParams>(params_)) {
+    branch = tensor(b);
+    if (!branch.defined() || !branch.is_cuda() || !branch.is_contiguous())
+      raise(PyExc_ValueError, "tensors must be contiguous CUDA tensors");
+    if (p.rows < 0 || p.channels < 0 || p.gate_groups < 0) raise(PyExc_ValueError, "negative extents");
+    numel = (int64_t)p.rows * p.channels;
+    dense(b, numel, branch, "branch");
+    post_gamma = dense(vectors[0], p.channels, branch, "post_gamma");
+    post_beta = dense(vectors[1], p.channels, branch, "post_beta");
+    gate = dense(vectors[2], (int64_t)p.gate_groups * p.channels, branch, "gate");
+    pre_gamma = dense(vectors[3], p.channels, branch, "pre_gamma");
+    pre_beta = dense(vectors[4], p.channels, branch, "pre_beta");
+  }
+  PdnnResidualNormTensors tensors() const {
+    PdnnResidualNormTensors t = {};
+    t.branch = ptr(branch);
+    t.post_gamma = ptr(post_gamma);
+    t.post_beta = ptr(post_beta);
+    t.gate = ptr(gate);
+    t.pre_gamma = ptr(pre_gamma);
+    t.pre_beta = ptr(pre_beta);
+    return t;
+  }
+};
+
+PyObject* residual_norm(PyObject* const* a) {
+  const NormTensors n(a[0], a[2], a + 3);
+  const at::Tensor residual = dense(a[1], n.numel, n.branch, "residual");
+  at::Tensor sum = dense(a[8], n.numel, n.branch, "sum_out"), out = dense(a[9], n.numel, n.branch, "out");
+  const int dtype = dtype_code(n.branch);
+  if (!sum.defined()) sum = like(n.branch);
+  if (!out.defined()) out = like(n.branch);
+  const at::Tensor statistics =
+      unlocked([&] { return at::empty({4, (int64_t)n.p.rows}, n.branch.options().dtype(at::kFloat)); });
+  PdnnResidualNormTensors t = n.tensors();
+  t.residual = ptr(residual);
+  t.sum = ptr(sum);
+  t.output = ptr(out);
+  t.statistics = static_cast<float*>(ptr(statistics));
+  const OnDevice on(n.branch);
+  call([&] { return pdnn_residual_norm(dtype, &n.p, &t, on.stream); });
+  return tuple_of({sum, out, statistics});
+}
+
+PyObject* residual_norm_grad(PyObject* const* a) {
+  const NormTensors n(a[2], a[5], a + 6);
+  const at::Tensor d_sum = dense(a[0], n.numel, n.branch, "sum_grad"), d_out = dense(a[1], n.numel, n.branch, "output_grad");
+  const at::Tensor sum = dense(a[3], n.numel, n.branch, "sum");
+  const at::Tensor statistics = dense(a[4], 4 * (int64_t)n.p.rows, n.branch, at::kFloat, "statistics");
+  if (!d_out.defined() || !sum.defined() || !statistics.defined()) raise(PyExc_ValueError, "output_grad, sum and statistics are needed");
+  at::Tensor d_branch = dense(a[11], n.numel, n.branch, "branch_grad"), d_residual = dense(a[12], n.numel, n.branch, "residual_grad");
+  const int dtype = dtype_code(n.branch);
+  if (!d_branch.defined()) d_branch = like(n.branch);
+  if (!d_residual.defined()) d_residual = like(n.branch);
+  const at::Tensor of[5] = {n.post_gamma, n.post_beta, n.gate, n.pre_gamma, n.pre_beta};
+  at::Tensor d[5];
+  for (int i = 0; i < 5; ++i)
+    if (of[i].defined()) d[i] = like(of[i]);
+  PdnnResidualNormTensors t = n.tensors();
+  t.sum = ptr(sum);
+  t.statistics = static_cast<float*>(ptr(statistics));
+  PdnnResidualNormGradients g = {};
+  g.sum_grad = ptr(d_sum);
+  g.output_grad = ptr(d_out);
+  g.branch_grad = ptr(d_branch);
+  g.residual_grad = ptr(d_residual);
+  g.post_gamma_grad = ptr(d[0]);
+  g.post_beta_grad = ptr(d[1]);
+  g.gate_grad = ptr(d[2]);
+  g.pre_gamma_grad = ptr(d[3]);
+  g.pre_beta_grad = ptr(d[4]);
+  const OnDevice on(n.branch);
+  call([&] { return pdnn_residual_norm_gradient(dtype, &n.p, &t, &g, on.stream); });
+  return tuple_of({d_branch, d_residual, d[0], d[1], d[2], d[3], d[4]});
+}
+
+PyObject* policy_loss(PyObject* const* a) {
+  const MatrixArg logits = matrix(a[0], "logits");
+  if (!logits.t.defined()) raise(PyExc_ValueError, "logits are needed");
+  const int dtype = dtype_code(logits.t);
+  const int64_t rows = logits.rows;
+  const at::Tensor targets = tensor(a[1]);
+  if (!targets.defined() || (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt))
+    raise(PyExc_ValueError, "targets must be a tensor of whole numbers of 32 or 64 bits");
+  dense(a[1], rows, logits.t, targets.scalar_type(), "targets");
+  const at::Tensor advantages = dense(a[2], rows, logits.t, at::kFloat, "advantages"),
+                   old_logp = dense(a[3], rows, logits.t, at::kFloat, "old_logp"),
+                   ref_logp = dense(a[4], rows, logits.t, at::kFloat, "ref_logp"),
+                   weights = dense(a[5], rows, logits.t, at::kFloat, "weights");
+  if (!advantages.defined()) raise(PyExc_ValueError, "advantages are needed");
+  PdnnPolicyLossParams p = {};
+  p.rows = extent(rows);
+  p.vocab = extent(logits.cols);
+  p.target_bytes = (int)targets.element_size();
+  p.clip_low = (float)real(a[6]);
+  p.clip_high = (float)real(a[7]);
+  p.kl = (float)real(a[8]);
+  p.temperature = (float)real(a[9]);
+  p.grad_scale = (float)real(a[10]);
+  const bool want_grad = truth(a[11]);
+  MatrixArg grad = matrix(a[12], "grad");
+  require_shape(grad, rows, logits.cols, logits.t, "grad");
+  if (!grad.t.defined() && want_grad) {
+    // dense, or in rows of whole packets where the logits' rows lie apart
+    const int64_t pitch = logits.pitch == logits.cols ? logits.cols : (logits.cols + 63) / 64 * 64;
+    grad = new_matrix(rows, pitch, logits.t);
+    grad.t = grad.t.narrow(1, 0, logits.cols);
+  }
+  p.logits_pitch = logits.pitch;
+  p.grad_pitch = grad.pitch;
+  const auto options = logits.t.options().dtype(at::kFloat);
+  const at::Tensor loss = unlocked([&] { return at::empty({}, options); }), token_loss = flat(rows, options), logp = flat(rows, options);
+  PdnnPolicyLossTensors t = {};
+  t.logits = ptr(logits.t);
+  t.targets = ptr(targets);
+  t.advantages = static_cast<const float*>(ptr(advantages));
+  t.old_logp = static_cast<const float*>(ptr(old_logp));
+  t.ref_logp = static_cast<const float*>(ptr(ref_logp));
+  t.weights = static_cast<const float*>(ptr(weights));
+  t.loss = static_cast<float*>(ptr(loss));
+  t.token_loss = static_cast<float*>(ptr(token_loss));
+  t.logp = static_cast<float*>(ptr(logp));
+  t.grad = ptr(grad.t);
+  const OnDevice on(logits.t);
+  call([&] { return pdnn_policy_loss(dtype, &p, &t, on.stream); });
+  return tuple_of({loss, token_loss, logp, grad.t});
+}
+
 // The CPython face of one of the functions above: argument count, C++ exceptions to Python ones.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -466,6 +745,11 @@ PyMethodDef kMethods[] = {ENTRY(conv2d, 17),
                           ENTRY(softmax, 7),
                           ENTRY(batchnorm_forward, 7),
                           ENTRY(batchnorm_gradient, 7),
+                          ENTRY(matmul_fused, 9),
+                          ENTRY(matmul_fused_grad, 15),
+                          ENTRY(residual_norm, 10),
+                          ENTRY(residual_norm_grad, 13),
+                          ENTRY(policy_loss, 13),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_front", "Native half of portdnn_b200.api.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

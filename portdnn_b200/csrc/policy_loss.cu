@@ -1,0 +1,319 @@
+// Clipped policy loss over the logits of a model's answers, with an estimate of the divergence from a reference
+// policy, forward and gradient in one call.  For token i with target t, logits x, temperature tau:
+//
+//   lp    = x_t / tau - log sum_j exp(x_j / tau)             log-probability of the token now
+//   ratio = exp(lp - old),  q = exp(ref - lp)
+//   loss  = -min(ratio * A, clip(ratio, 1 - low, 1 + high) * A) + kl * (q - 1 - (ref - lp))
+//   slope = d loss / d lp = -(ratio * A where that is the smaller one, else 0) + kl * (1 - q)
+//   grad_j = grad_scale * w / tau * slope * ([j = t] - p_j),   p_j = exp(x_j / tau) / sum
+//
+// Bound by memory: the logits are read once and the gradient written once.  The loss of a token depends on its whole
+// row, so that a block walks the row twice: once for the maximum and the sum - together, the sum scaled down whenever
+// the maximum rises - and once for the gradient.  The rows that the device works on at a time stay in the 126 MB L2
+// cache, from where the second walk reads them.  Few rows are split among the CTAs of a cluster, which exchange
+// maxima and sums through distributed shared memory and add them in the order of their ranks.
+#include "common.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace pdnn {
+namespace {
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+struct LossArgs {
+  const void *logits, *targets;
+  const float *advantages, *old_logp, *ref_logp, *weights;
+  float *token_loss, *logp;
+  void* grad;
+  int rows, vocab, wide_targets, packets;
+  long long pitch, grad_pitch;
+  float c, inv_temperature, clip_low, clip_high, kl, grad_scale;  // c = log2(e) / temperature
+};
+
+// The largest value so far and the sum of 2^((v - top) * c).  Of values that are all minus infinity the sum is 0.
+struct alignas(8) Partial {
+  float top, sum;
+};
+__device__ __forceinline__ Partial merge(Partial a, Partial b, float c) {
+  const float top = fmaxf(a.top, b.top);
+  // (equal tops, infinite ones among them, need no scaling; NaN sums stay NaN)
+  const float fa = a.top == top ? 1.f : exp2_fast((a.top - top) * c), fb = b.top == top ? 1.f : exp2_fast((b.top - top) * c);
+  return Partial{top, a.sum * fa + b.sum * fb};
+}
+
+template <typename T>
+__device__ __forceinline__ void store_streaming(T* p, const Vec16<T>& v) {
+  __stcs(reinterpret_cast<uint4*>(p), v.raw);
+}
+
+// One row to a cluster of CTAs (most often to a CTA).
+template <typename T>
+__global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
+  overlap_wait();
+  constexpr int N = Vec16<T>::N, kUnroll = 4;
+  __shared__ Partial warp_part[16];
+  __shared__ Partial cta_part;
+  __shared__ float shared_slope;
+  const int threads = (int)blockDim.x, tid = (int)threadIdx.x;
+  uint32_t ranks, rank;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int row = (int)(blockIdx.x / ranks);
+  const T* x = static_cast<const T*>(a.logits) + (size_t)row * a.pitch;
+  T* g = a.grad != nullptr ? static_cast<T*>(a.grad) + (size_t)row * a.grad_pitch : nullptr;
+  // this CTA's share of the row, whole packets but for the end
+  const int share = ((a.vocab + (int)ranks - 1) / (int)ranks + N - 1) / N * N;
+  const int begin = min((int)rank * share, a.vocab), end = min(begin + share, a.vocab);
+  const int packed_end = a.packets ? begin + (end - begin) / N * N : begin;
+  const long long t = a.wide_targets ? static_cast<const long long*>(a.targets)[row] : (long long)static_cast<const int*>(a.targets)[row];
+  const float weight = a.weights != nullptr ? a.weights[row] : 1.f;
+  // A row without weight or without a token counts for nothing, whatever stands in it: it is not read.
+  const bool counts = weight != 0.f && t >= 0 && t < a.vocab;
+  if (!counts) {
+    if (rank == 0 && tid == 0) {
+      a.token_loss[row] = 0.f;
+      a.logp[row] = 0.f;
+    }
+    if (g != nullptr) {
+      Vec16<T> zero;
+      zero.raw = make_uint4(0u, 0u, 0u, 0u);
+      for (int j = begin + tid * N; j < packed_end; j += threads * N) store_streaming(g + j, zero);
+      for (int j = packed_end + tid; j < end; j += threads) g[j] = from_f32<T>(0.f);
+    }
+    return;  // (all CTAs of the cluster alike)
+  }
+
+  // (read ahead of every write: the gradient may take the place of the logits)
+  const float chosen = tid == 0 ? to_f32(x[t]) : 0.f;
+  Partial part{-INFINITY, 0.f};
+  auto take = [&](const float* v, int n) {
+    float top = part.top;
+    for (int i = 0; i < n; ++i) top = fmaxf(top, v[i]);
+    if (top > part.top) {
+      part.sum *= exp2_fast((part.top - top) * a.c);  // (from minus infinity: 0 times 0)
+      part.top = top;
+    }
+    if (part.top == -INFINITY) {  // nothing but minus infinity, or NaN, which fmaxf passes over
+      for (int i = 0; i < n; ++i)
+        if (v[i] != v[i]) part.sum = v[i];
+      return;
+    }
+    float sum = 0.f;
+    for (int i = 0; i < n; ++i) sum += exp2_fast((v[i] - part.top) * a.c);
+    part.sum += sum;
+  };
+  {
+    int j = begin + tid * N;
+    for (; j + (kUnroll - 1) * threads * N < packed_end; j += kUnroll * threads * N) {
+      Vec16<T> p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * threads * N);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_f32(p[u].get(i));
+        take(v, N);
+      }
+    }
+    for (; j < packed_end; j += threads * N) {
+      const Vec16<T> p = load16(x + j);
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = to_f32(p.get(i));
+      take(v, N);
+    }
+    for (int k = packed_end + tid; k < end; k += threads) {
+      const float v = to_f32(x[k]);
+      take(&v, 1);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Partial other{__shfl_xor_sync(0xFFFFFFFFu, part.top, o), __shfl_xor_sync(0xFFFFFFFFu, part.sum, o)};
+    part = merge(part, other, a.c);
+  }
+  if ((tid & 31) == 0) warp_part[tid >> 5] = part;
+  __syncthreads();
+  part = warp_part[0];
+  for (int w = 1; w < threads / 32; ++w) part = merge(part, warp_part[w], a.c);
+  if (ranks > 1) {
+    if (tid == 0) cta_part = part;
+    umma::cluster_sync_all();
+    const uint32_t mine = umma::smem_u32(&cta_part);
+    for (uint32_t r = 0; r < ranks; ++r) {
+      Partial other;
+      const uint32_t at = umma::cluster_map_shared(mine, r);
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(other.top), "=f"(other.sum) : "r"(at) : "memory");
+      part = r == 0 ? other : merge(part, other, a.c);
+    }
+    umma::cluster_sync_all();  // nobody leaves while its sums are read
+  }
+  if (tid == 0) {
+    float slope = 0.f, loss = 0.f, lp = 0.f;
+    if (!(part.top == -INFINITY && part.sum == 0.f)) {  // (a row of nothing but minus infinity counts for nothing)
+      lp = (chosen - part.top) * a.inv_temperature - log2f(part.sum) * kLn2;
+      const float adv = a.advantages[row];
+      const float ratio = a.old_logp != nullptr ? expf(lp - a.old_logp[row]) : 1.f;
+      const float open = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * adv;
+      loss = -fminf(open, clipped);
+      slope = open <= clipped ? -open : 0.f;
+      if (open != open) loss = slope = open;
+      if (a.ref_logp != nullptr) {
+        const float d = a.ref_logp[row] - lp, q = expf(d);
+        loss += a.kl * (q - d - 1.f);
+        slope += a.kl * (1.f - q);
+      }
+      loss *= weight;
+      slope *= weight * a.grad_scale * a.inv_temperature;
+    }
+    shared_slope = slope;
+    if (rank == 0) {
+      a.token_loss[row] = loss;
+      a.logp[row] = lp;
+    }
+  }
+  if (g == nullptr) return;
+  __syncthreads();
+  const float slope = shared_slope, top = part.top == -INFINITY ? 0.f : part.top;
+  const float k = part.sum == 0.f ? 0.f : -slope / part.sum;
+  const int target = (int)t;
+  auto gradient = [&](float v, int j) { return exp2_fast((v - top) * a.c) * k + (j == target ? slope : 0.f); };
+  {
+    int j = begin + tid * N;
+    for (; j + (kUnroll - 1) * threads * N < packed_end; j += kUnroll * threads * N) {
+      Vec16<T> p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * threads * N);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        Vec16<T> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.set(i, from_f32<T>(gradient(to_f32(p[u].get(i)), j + u * threads * N + i)));
+        store_streaming(g + j + u * threads * N, o);
+      }
+    }
+    for (; j < packed_end; j += threads * N) {
+      const Vec16<T> p = load16(x + j);
+      Vec16<T> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.set(i, from_f32<T>(gradient(to_f32(p.get(i)), j + i)));
+      store_streaming(g + j, o);
+    }
+    for (int j1 = packed_end + tid; j1 < end; j1 += threads) g[j1] = from_f32<T>(gradient(to_f32(x[j1]), j1));
+  }
+}
+
+// The sum of the tokens' losses, in one order.
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* token_loss, int rows, float* loss) {
+  overlap_wait();
+  __shared__ float warp_sums[32];
+  float sum = 0.f;
+  for (int i = (int)threadIdx.x; i < rows; i += 1024) sum += token_loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sum = warp_sums[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (threadIdx.x == 0) *loss = sum;
+  }
+}
+
+template <typename T>
+void launch_rows(const LossArgs& a, int cluster, int threads, cudaStream_t s) {
+  const dim3 grid((unsigned)a.rows * (unsigned)cluster);
+  if (cluster == 1) {
+    launch_overlapped(policy_loss_kernel<T>, grid, (unsigned)threads, s, a);
+    return;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, policy_loss_kernel<T>, a);  // (the caller's check_launch() reads the error)
+}
+
+}  // namespace
+
+int launch_policy_loss(int dtype, const PdnnPolicyLossParams& p, const PdnnPolicyLossTensors& t, cudaStream_t s) {
+  const char* what = "policy loss";
+  if (dtype < PDNN_F32 || dtype > PDNN_BF16) return fail(PDNN_INVALID_PARAMETER, "%s: unknown dtype %d", what, dtype);
+  if (p.rows < 0 || p.vocab <= 0) return fail(PDNN_INVALID_PARAMETER, "%s: %d rows of %d logits", what, p.rows, p.vocab);
+  if (p.vocab > 1 << 30) return fail(PDNN_INDEX_EXCEEDED, "%s: rows of more than 2^30 logits", what);
+  if (p.logits_pitch < p.vocab || (t.grad != nullptr && p.grad_pitch < p.vocab))
+    return fail(PDNN_INVALID_PARAMETER, "%s: a row's pitch is shorter than the row", what);
+  if (p.target_bytes != 4 && p.target_bytes != 8)
+    return fail(PDNN_INVALID_PARAMETER, "%s: targets are whole numbers of 4 or 8 bytes", what);
+  if (!(p.temperature > 0.f) || std::isinf(p.temperature))
+    return fail(PDNN_INVALID_PARAMETER, "%s: the temperature must be positive", what);
+  if (!(p.clip_low >= 0.f) || !(p.clip_high >= 0.f))
+    return fail(PDNN_INVALID_PARAMETER, "%s: clipping bounds must not be negative", what);
+  if (t.loss == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  if (p.rows > 0 && (t.logits == nullptr || t.targets == nullptr || t.advantages == nullptr || t.token_loss == nullptr || t.logp == nullptr))
+    return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  const int sms = device_sm_count();
+  if (sms <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
+  if (p.rows > 0) {
+    const long long es = (long long)dtype_size(dtype);
+    LossArgs a = {};
+    a.logits = t.logits;
+    a.targets = t.targets;
+    a.advantages = t.advantages;
+    a.old_logp = t.old_logp;
+    a.ref_logp = t.ref_logp;
+    a.weights = t.weights;
+    a.token_loss = t.token_loss;
+    a.logp = t.logp;
+    a.grad = t.grad;
+    a.rows = p.rows;
+    a.vocab = p.vocab;
+    a.wide_targets = p.target_bytes == 8;
+    a.pitch = p.logits_pitch;
+    a.grad_pitch = p.grad_pitch;
+    a.packets = aligned16(t.logits) && p.logits_pitch * es % 16 == 0 &&
+                (t.grad == nullptr || (aligned16(t.grad) && p.grad_pitch * es % 16 == 0));
+    a.inv_temperature = 1.f / p.temperature;
+    a.c = kLog2e / p.temperature;
+    a.clip_low = p.clip_low;
+    a.clip_high = p.clip_high;
+    a.kl = p.kl;
+    a.grad_scale = p.grad_scale;
+    // A packet to a thread and walk, at most 512 threads; rows in shares of at least a walk of 128 threads while the device
+    // has room for more blocks.
+    const long long packets = ((long long)p.vocab * es + 15) / 16;
+    int cluster = 1;
+    while (cluster < 8 && (long long)p.rows * cluster * 2 <= 2ll * sms && packets / (cluster * 2) >= 128) cluster *= 2;
+    int threads = 128;
+    while (threads < 512 && packets / cluster > 2 * threads) threads *= 2;
+    if (dtype == PDNN_F32) launch_rows<float>(a, cluster, threads, s);
+    if (dtype == PDNN_F16) launch_rows<__half>(a, cluster, threads, s);
+    if (dtype == PDNN_BF16) launch_rows<__nv_bfloat16>(a, cluster, threads, s);
+    const int st = check_launch(what);
+    if (st != PDNN_OK) return st;
+  }
+  launch_overlapped(loss_sum_kernel, 1, 1024, s, t.token_loss, p.rows, t.loss);
+  return check_launch("policy loss sum");
+}
+
+}  // namespace pdnn
