@@ -1,0 +1,1120 @@
+// D = A * B on the 5th-generation tensor cores with the end of a fully connected layer in the same kernel: bias,
+// activation, residual and a copy of the pre-activation on the way forward, the slope of the preceding activation on the
+// way back.  A is M x K, B is N x K, either of them K-major (rows of K) or MN-major (rows of M or N), so that the layer, its
+// input gradient and its weight gradient read the caller's tensors as they lie, slices of wider ones among them.
+//
+// pair_gemm_kernel: tiles of 256 x 256 (or 256 x 128) on clusters of two CTAs, persistent, for products that have a tile
+// for most of the SM pairs.  solo_gemm_kernel: tiles of 128 x up to 128, whose steps a cluster of up to eight CTAs shares,
+// for all others; a few rows of tokens become the columns of the tile, so that the weights fill its 128 rows.
+//
+// fp32: the tensor cores' fp32 accumulator drops the bits below its last place instead of rounding them, an error that
+// grows with the number of additions and has one sign (k = 515 in three TF32 products a term: 3.9e-6 of the result, ten times
+// that of fp32 multiply-adds).  So operands are cut into three bf16 parts (8 bits each, 24 in all; the three smallest of
+// the nine products, below 2^-24, are left out), and a chain ends after every 64 terms: the epilogue warps add what
+// the accumulator holds to sums of their own, rounded to nearest, while the other accumulator takes the next 64.
+#include "fused_gemm.cuh"
+
+#include "activation.cuh"
+#include "tc_gemm.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+namespace pdnn {
+namespace {
+
+using namespace umma;
+
+constexpr int kStepK = 64;         // reduction elements of a stage: a 128-byte row of 16-bit elements
+constexpr int kMostStages = 12;
+constexpr int kSlotBytes = 4096;   // 32 rows of 128 bytes, swizzled as TMA does
+constexpr int kSmemBudget = 232448;
+constexpr int kParts = 6;          // products of parts that make an fp32 product
+
+struct alignas(64) FusedArgs {
+  CUtensorMap a_map, b_map, out_map, aux_map, pre_map;
+  Finish f;
+  unsigned* error_record;
+  uint64_t wait_limit_ns;
+  int tiles_m, tiles_n, group_m;     // tiles; rows of tiles that are walked together
+  int kblocks, part_k;               // steps along K (of each product of parts); distance between two parts along K
+  int a_mn, b_mn, stages;
+  unsigned a_lbo, a_sbo, a_kadv, b_lbo, b_sbo, b_kadv, idesc;
+  int out_tma, aux_tma, pre_tma;
+  // solo_gemm_kernel
+  int bn, splits, blocks_per_split, swapped, tmem_cols;
+  int out_vec, aux_vec, pre_vec, bias_vec;  // four elements at a time
+};
+
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+               : "memory");
+}
+// (the barrier of the pair's first CTA counts the bytes)
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar & kPeerBitMask), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// A wait of the whole warp: all lanes learn the same, so that none is left behind at a warp barrier when one gives up.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const FusedArgs& a, unsigned where) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, a.error_record, a.wait_limit_ns, where));
+}
+
+// The product of parts that step `part` takes: first the largest.
+__device__ __forceinline__ int part_of_a(int part) { return part == 2 || part == 3 ? 1 : part == 5 ? 2 : 0; }
+__device__ __forceinline__ int part_of_b(int part) { return part == 1 || part == 3 ? 1 : part == 4 ? 2 : 0; }
+
+// Where element byte `b` of row `r` of a slot is.
+__device__ __forceinline__ uint32_t slot_at(int r, int b) { return (uint32_t)(r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15))); }
+
+// Phi(z), the normal distribution's function: a polynomial in 1 / (1 + p |x|) times exp(-x^2), x = z / sqrt(2) (Abramowitz and
+// Stegun, 7.1.26; off by 7.5e-8 at most, in the tail relative to exp(-x^2)).  For results of 16 bits.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678f;
+  const float t = __fdividef(1.f, 1.f + 0.3275911f * x);
+  e = __expf(-x * x);
+  const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z >= 0.f ? 1.f - q : q;
+}
+
+// The activation ACT, and its slope, for a result of type OutT.
+template <int ACT, typename OutT>
+__device__ __forceinline__ float value_of(float z) {
+  if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_GELU) {
+    float e;
+    return z * normal_cdf(z, e);
+  } else if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_SILU) {
+    return __fdividef(z, 1.f + __expf(-z));
+  } else {
+    return activate(ACT, z);
+  }
+}
+template <int ACT, typename OutT>
+__device__ __forceinline__ float slope_of(float z) {
+  if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_GELU) {
+    float e;
+    const float c = normal_cdf(z, e);
+    return c + z * 0.39894228f * e;
+  } else {
+    return activation_slope(ACT, z);
+  }
+}
+
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  switch (act) {
+    case PDNN_ACT_RELU: f(std::integral_constant<int, PDNN_ACT_RELU>{}); break;
+    case PDNN_ACT_TANH: f(std::integral_constant<int, PDNN_ACT_TANH>{}); break;
+    case PDNN_ACT_RELU6: f(std::integral_constant<int, PDNN_ACT_RELU6>{}); break;
+    case PDNN_ACT_GELU: f(std::integral_constant<int, PDNN_ACT_GELU>{}); break;
+    case PDNN_ACT_SILU: f(std::integral_constant<int, PDNN_ACT_SILU>{}); break;
+    case PDNN_ACT_SIGMOID: f(std::integral_constant<int, PDNN_ACT_SIGMOID>{}); break;
+    default: f(std::integral_constant<int, PDNN_ACT_NONE>{}); break;
+  }
+}
+
+// A 16-byte chunk of a slot as floats, and back.
+template <typename OutT>
+__device__ __forceinline__ void unpack(uint4 q, float* v) {
+  Vec16<OutT> p;
+  p.raw = q;
+#pragma unroll
+  for (int i = 0; i < Vec16<OutT>::N; ++i) v[i] = to_f32(p.get(i));
+}
+template <typename OutT>
+__device__ __forceinline__ uint4 pack(const float* v) {
+  if constexpr (sizeof(OutT) == 4) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  } else if constexpr (std::is_same<OutT, __half>::value) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// A slot's 32 rows from or to memory that TMA cannot reach (off a 16-byte boundary), neighbouring lanes on neighbouring
+// elements.
+template <typename OutT>
+__device__ __forceinline__ void slot_from_memory(uint8_t* slot, const OutT* from, long long pitch, int rows, int cols, int lane) {
+  constexpr int CB = 128 / (int)sizeof(OutT);
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r)
+#pragma unroll
+    for (int c = lane; c < CB; c += 32)
+      if (r < rows && c < cols) *reinterpret_cast<OutT*>(slot + slot_at(r, c * (int)sizeof(OutT))) = from[(long long)r * pitch + c];
+}
+template <typename OutT>
+__device__ __forceinline__ void slot_to_memory(const uint8_t* slot, OutT* to, long long pitch, int rows, int cols, int lane) {
+  constexpr int CB = 128 / (int)sizeof(OutT);
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r)
+#pragma unroll
+    for (int c = lane; c < CB; c += 32)
+      if (r < rows && c < cols) to[(long long)r * pitch + c] = *reinterpret_cast<const OutT*>(slot + slot_at(r, c * (int)sizeof(OutT)));
+}
+
+// ------------------------------------------------------------------------------------------------
+// Clusters of two CTAs.  A tile is 256 rows x BN columns: each CTA loads its own 128 rows of A and half of the columns of B
+// to a stage, rank 0 issues the MMAs of 256 x BN x 16 that read both shared memories, and each CTA finds its 128 rows of the
+// accumulator in its own tensor memory, in one of two buffers, so that the end of a tile overlaps the MMAs of the
+// next.  Warp 0 loads, warp 1 issues, warps 2 to 9 make the ends: 32 rows and half of the columns each, 128 bytes of a row at a time
+// through a slot of shared memory that TMA fills (residual or slope argument) and empties.
+// Bound by the tensor cores with shared memory close behind (64 bytes a cycle of operands and 64 of fills).
+// ------------------------------------------------------------------------------------------------
+constexpr int kPairThreads = 320, kEndWarps = 8;
+
+template <typename OutT, int BN, bool SPLIT>
+__global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid_constant__ FusedArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  const FusedArgs& a = args;
+  constexpr uint32_t kABytes = 128u * 128u, kBBytes = (uint32_t)(BN / 2) * 128u, kStage = kABytes + kBBytes;
+  constexpr int CB = 128 / (int)sizeof(OutT), kCols = BN / 2, kBlocks = kCols / CB;  // columns of a block, of a warp; blocks of a warp
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = (int)(threadIdx.x & 31);
+  const uint32_t rank = cluster_cta_rank();
+  const bool leader = rank == 0;
+  const int S = a.stages;
+  const uint32_t slots_off = (uint32_t)S * kStage, bar_off = slots_off + 2u * kEndWarps * kSlotBytes;
+  const uint32_t bars = base + bar_off;
+  auto full_bar = [&](int s) { return bars + 8u * (uint32_t)s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (uint32_t)(kMostStages + s); };
+  auto acc_full_bar = [&](int b) { return bars + 8u * (uint32_t)(2 * kMostStages + b); };
+  auto acc_empty_bar = [&](int b) { return bars + 8u * (uint32_t)(2 * kMostStages + 2 + b); };
+  auto aux_bar = [&](int w, int b) { return bars + 8u * (uint32_t)(2 * kMostStages + 4 + 2 * w + b); };
+  constexpr int kBars = 2 * kMostStages + 4 + 2 * kEndWarps;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + bar_off + 8 * kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + bar_off + 8 * kBars + 4);
+  uint8_t* bias_strips = smem + bar_off + 8 * kBars + 16;  // 128 bytes a warp
+
+  if ((int)threadIdx.x < kBars) {
+    const int j = (int)threadIdx.x;
+    mbar_init(bars + 8u * (uint32_t)j, j == 2 * kMostStages + 2 || j == 2 * kMostStages + 3 ? 2u * kEndWarps : 1u);
+    if (j == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&a.a_map);
+    prefetch_tensormap(&a.b_map);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 2u * BN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();  // the peer's barriers are initialised before anything signals them
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = a.tiles_m * a.tiles_n, first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+  // a band of group_m rows of tiles is walked column by column, so that the tiles in flight share rows and columns
+  auto tile_at = [&](int tile, int& m0, int& n0) {
+    const int per = a.group_m * a.tiles_n, band = tile / per, rest = tile - band * per;
+    const int high = min(a.group_m, a.tiles_m - band * a.group_m), nt = rest / high;
+    m0 = (band * a.group_m + rest - nt * high) * 256 + (int)rank * 128;
+    n0 = nt * BN;
+  };
+  const int parts = SPLIT ? kParts : 1;
+
+  if (warp == 0) {
+    // ------------------------------- producer ------------------------------------------------
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    grid_dependency_wait();
+#pragma unroll 1
+    for (int tile = first; tile < total && ok; tile += step) {
+      int m0, n0;
+      tile_at(tile, m0, n0);
+      n0 += (int)rank * (BN / 2);
+#pragma unroll 1
+      for (int kb = 0; kb < a.kblocks && ok; ++kb)
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part) {
+          if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x1100u + (unsigned)s)) {
+            ok = false;
+            break;
+          }
+          const uint32_t fb = full_bar(s), sa = base + (uint32_t)s * kStage, sb = sa + kABytes;
+          const int ka = kb * kStepK + (SPLIT ? part_of_a(part) * a.part_k : 0), kc = kb * kStepK + (SPLIT ? part_of_b(part) * a.part_k : 0);
+          if (elect_one()) {
+            if (leader) mbar_arrive_expect_tx(fb, 2u * kStage);  // the bytes of both CTAs
+            if (a.a_mn) {
+              load_2d_pair(sa, &a.a_map, fb, m0, ka);
+              load_2d_pair(sa + 8192u, &a.a_map, fb, m0 + 64, ka);
+            } else {
+              load_2d_pair(sa, &a.a_map, fb, ka, m0);
+            }
+            if (a.b_mn) {
+              load_2d_pair(sb, &a.b_map, fb, n0, kc);
+              if (BN == 256) load_2d_pair(sb + 8192u, &a.b_map, fb, n0 + 64, kc);
+            } else {
+              load_2d_pair(sb, &a.b_map, fb, kc, n0);
+            }
+          }
+          __syncwarp();
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+    }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer (rank 0) --------------------------------------
+    grid_dependency_wait();
+    grid_launch_dependents();  // the grid is a single wave, and its columns of tensor memory are taken
+    if (leader) {
+      const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo);
+      const uint32_t a_kadv = a.a_kadv >> 4, b_kadv = a.b_kadv >> 4, idesc = a.idesc;
+      const int chains = SPLIT ? a.kblocks : 1, steps = SPLIT ? kParts : a.kblocks;  // accumulator fills of a tile, steps of each
+      int s = 0;
+      uint32_t ph = 0, buf = 0, aph = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int tile = first; tile < total && ok; tile += step)
+#pragma unroll 1
+        for (int chain = 0; chain < chains && ok; ++chain) {
+          if (!warp_wait(acc_empty_bar((int)buf), aph ^ 1u, abort_flag, a, 0x1200u + buf)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t d = tmem_base + buf * (uint32_t)BN;
+          uint32_t accumulate = 0u;
+#pragma unroll 1
+          for (int ks = 0; ks < steps; ++ks) {
+            if (!warp_wait(full_bar(s), ph, abort_flag, a, 0x1300u + (unsigned)s)) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = (base + (uint32_t)s * kStage) & 0x3FFFFu;  // offset inside the CTA's shared memory
+            const uint64_t da = a_desc0 + (uint64_t)(sa >> 4), db = b_desc0 + (uint64_t)((sa + kABytes) >> 4);
+            warp_mma_f16_pair(d, da, db, idesc, accumulate);
+            warp_mma_f16_pair(d, da + a_kadv, db + b_kadv, idesc, 1u);
+            warp_mma_f16_pair(d, da + 2 * a_kadv, db + 2 * b_kadv, idesc, 1u);
+            warp_mma_f16_pair(d, da + 3 * a_kadv, db + 3 * b_kadv, idesc, 1u);
+            accumulate = 1u;
+            warp_commit_pair(empty_bar(s), cluster_map_shared(empty_bar(s), 1u));  // both CTAs may refill the stage
+            if (++s == S) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+          if (!ok) break;
+          warp_commit_pair(acc_full_bar((int)buf), cluster_map_shared(acc_full_bar((int)buf), 1u));
+          if (++buf == 2u) {
+            buf = 0;
+            aph ^= 1u;
+          }
+        }
+    }
+  } else {
+    // ------------------------------- ends (own 128 rows) --------------------------------------
+    const int w = warp - 2, q = warp & 3, half = w >> 2;  // tensor memory lanes [32 q, 32 q + 32)
+    uint8_t* slots = smem + slots_off + (size_t)w * 2 * kSlotBytes;
+    const uint32_t slots_addr = base + slots_off + (uint32_t)w * 2u * kSlotBytes;
+    OutT* strip = reinterpret_cast<OutT*>(bias_strips + w * 128);
+    const Finish& f = a.f;
+    const bool has_aux = f.aux != nullptr, has_pre = f.pre != nullptr;
+    // Blocks take the two slots in turn; where the pre-activation is stored, too, it has the second one to itself.
+    uint32_t blocks_done = 0, aux_phase = 0u, buf = 0, aph = 0;
+    grid_dependency_wait();
+    bool ok = true;
+#pragma unroll 1
+    for (int tile = first; tile < total && ok; tile += step) {
+      int m0, n0;
+      tile_at(tile, m0, n0);
+      const int row0 = m0 + q * 32, col0 = n0 + half * kCols, rows_left = f.rows - row0;
+      auto slot_of = [&](int block) { return has_pre ? 0 : (int)((blocks_done + (uint32_t)block) & 1u); };
+      auto request_aux = [&](int block) {  // into its slot, whose last store has been read by now
+        const int col = col0 + block * CB;
+        if (!has_aux || col >= f.cols || rows_left <= 0) return;
+        const int slot = slot_of(block);
+        if (a.aux_tma) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(aux_bar(w, slot), kSlotBytes);
+            load_2d(slots_addr + (uint32_t)slot * kSlotBytes, &a.aux_map, aux_bar(w, slot), col, row0);
+          }
+        } else {
+          slot_from_memory<OutT>(slots + slot * kSlotBytes, static_cast<const OutT*>(f.aux) + (long long)row0 * f.aux_pitch + col,
+                                 f.aux_pitch, rows_left, f.cols - col, lane);
+        }
+      };
+      auto bias_at = [&](int block, float (&b)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = col0 + block * CB + lane + 32 * i;
+          b[i] = f.bias != nullptr && 32 * i < CB && c < f.cols ? to_f32(static_cast<const OutT*>(f.bias)[c]) : 0.f;
+        }
+      };
+      float bias[2];
+      bias_at(0, bias);
+      if (lane == 0) bulk_wait_group_read<0>();
+      __syncwarp();
+      request_aux(0);
+      float sums[SPLIT ? kCols : 1];
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) sums[i] = 0.f;
+#pragma unroll 1
+        for (int chain = 0; chain < a.kblocks; ++chain) {
+          if (!warp_wait(acc_full_bar((int)buf), aph, abort_flag, a, 0x1400u + buf)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)BN + (uint32_t)(half * kCols);
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32(acc + (uint32_t)c, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sums[c + i] += __uint_as_float(r[i]);
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_empty_bar((int)buf) & kPeerBitMask);  // rank 0 collects both CTAs
+          if (++buf == 2u) {
+            buf = 0;
+            aph ^= 1u;
+          }
+        }
+        if (!ok) break;
+      } else {
+        if (!warp_wait(acc_full_bar((int)buf), aph, abort_flag, a, 0x1400u + buf)) break;
+        tc_fence_after_sync();
+      }
+      const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + buf * (uint32_t)BN + (uint32_t)(half * kCols);
+#pragma unroll 1
+      for (int block = 0; block < kBlocks; ++block) {
+        const int col = col0 + block * CB, slot = slot_of(block);
+        const bool inside = col < f.cols && rows_left > 0;
+        float v[CB];
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)  // (registers are not indexed at run time)
+            if (b == block) {
+#pragma unroll
+              for (int i = 0; i < CB; ++i) v[i] = sums[b * CB + i];
+            }
+        } else {
+          uint32_t r[CB / 32][32];
+#pragma unroll
+          for (int c = 0; c < CB / 32; ++c) tmem_ld_32x32(acc + (uint32_t)(block * CB + c * 32), r[c]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < CB; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
+          if (block + 1 == kBlocks) {  // the accumulator is free
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty_bar((int)buf) & kPeerBitMask);
+          }
+        }
+        if (f.bias != nullptr) {
+          __syncwarp();
+          strip[lane] = from_f32<OutT>(bias[0]);
+          if (CB > 32) strip[lane + 32] = from_f32<OutT>(bias[1]);
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < CB; c += Vec16<OutT>::N) {
+            float b[Vec16<OutT>::N];
+            unpack<OutT>(*reinterpret_cast<const uint4*>(strip + c), b);
+#pragma unroll
+            for (int i = 0; i < Vec16<OutT>::N; ++i) v[c + i] += b[i];
+          }
+        }
+        if (block + 1 < kBlocks) bias_at(block + 1, bias);
+        uint8_t* my_row = slots + slot * kSlotBytes + lane * 128;
+        if (has_aux && inside) {
+          if (a.aux_tma) {
+            if (!warp_wait(aux_bar(w, slot), (aux_phase >> slot) & 1u, abort_flag, a, 0x1500u + (unsigned)slot)) {
+              ok = false;
+              break;
+            }
+            aux_phase ^= 1u << slot;
+          } else {
+            __syncwarp();
+          }
+        }
+        // the slots of the next block: their stores have been read
+        if (lane == 0 && !has_pre) bulk_wait_group_read<0>();
+        __syncwarp();
+        if (block + 1 < kBlocks && !has_pre) request_aux(block + 1);
+        if (inside) {
+          if (has_pre) {
+            uint8_t* pre_row = slots + kSlotBytes + lane * 128;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(pre_row + ((j ^ (lane & 7)) << 4)) = pack<OutT>(v + j * Vec16<OutT>::N);
+          }
+          with_activation(f.act, [&](auto act) {
+            constexpr int ACT = decltype(act)::value, N = Vec16<OutT>::N;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint4* at = reinterpret_cast<uint4*>(my_row + ((j ^ (lane & 7)) << 4));
+              float x[N];
+              if (has_aux) unpack<OutT>(*at, x);
+#pragma unroll
+              for (int i = 0; i < N; ++i) {
+                float& o = v[j * N + i];
+                if (f.gradient) {
+                  if (has_aux) o *= slope_of<ACT, OutT>(x[i]);
+                } else {
+                  o = f.scale * value_of<ACT, OutT>(o);
+                  if (has_aux) o += x[i];
+                }
+              }
+              *at = pack<OutT>(v + j * N);
+            }
+          });
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (has_pre) {
+            if (a.pre_tma) {
+              if (lane == 0) store_2d(&a.pre_map, slots_addr + kSlotBytes, col, row0);
+            } else {
+              slot_to_memory<OutT>(slots + kSlotBytes, static_cast<OutT*>(f.pre) + (long long)row0 * f.pre_pitch + col, f.pre_pitch,
+                                   rows_left, f.cols - col, lane);
+            }
+          }
+          if (a.out_tma) {
+            if (lane == 0) store_2d(&a.out_map, slots_addr + (uint32_t)slot * kSlotBytes, col, row0);
+          } else {
+            slot_to_memory<OutT>(slots + slot * kSlotBytes, static_cast<OutT*>(f.out) + (long long)row0 * f.out_pitch + col,
+                                 f.out_pitch, rows_left, f.cols - col, lane);
+          }
+          if (lane == 0) bulk_commit_group();
+          __syncwarp();
+        }
+        if (has_pre && block + 1 < kBlocks) {  // both slots are needed again
+          if (lane == 0) bulk_wait_group_read<0>();
+          __syncwarp();
+          request_aux(block + 1);
+        }
+      }
+      if (!ok) break;
+      blocks_done += kBlocks;
+      if constexpr (!SPLIT) {
+        if (++buf == 2u) {
+          buf = 0;
+          aph ^= 1u;
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group_read<0>();
+  }
+
+  // ------------------------------- teardown ---------------------------------------------------
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {  // copies already issued may still be landing in shared memory
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) {
+    }
+    __syncthreads();
+  }
+  cluster_sync_all();  // neither CTA leaves while the other may still use its shared and tensor memory
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 2u * BN);
+}
+
+// ------------------------------------------------------------------------------------------------
+// One tile of 128 x bn to a cluster of `splits` CTAs, each of which takes a share of the steps along K.  Partial tiles go to
+// shared memory, where each CTA of the cluster adds up its share of the tile's rows in the order of the ranks and finishes
+// them, four neighbouring elements to a thread.  swapped: the tile's rows are the columns of the result.  Two CTAs fit
+// an SM, so that the end of one overlaps the loads of another.
+// ------------------------------------------------------------------------------------------------
+constexpr int kSoloThreads = 192, kSoloSmem = 110 * 1024, kSoloHead = 2048, kSplitCols = 64;
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four neighbouring elements of a row, `left` of them inside it.
+template <typename OutT>
+__device__ __forceinline__ void load_four(const OutT* p, bool vec, int left, float (&v)[4]) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(OutT) == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p);
+      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      const OutT* e = reinterpret_cast<const OutT*>(&q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+  }
+}
+template <typename OutT>
+__device__ __forceinline__ void store_four(OutT* p, bool vec, int left, const float (&v)[4]) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(OutT) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint2 q;
+      OutT* e = reinterpret_cast<OutT*>(&q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = from_f32<OutT>(v[i]);
+      *reinterpret_cast<uint2*>(p) = q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = from_f32<OutT>(v[i]);
+  }
+}
+
+template <typename OutT, bool SPLIT>
+__global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid_constant__ FusedArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  const FusedArgs& a = args;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = (int)(threadIdx.x & 31);
+  const int splits = a.splits, rank = (int)blockIdx.x % splits, tile = (int)blockIdx.x / splits;
+  const int S = a.stages, bn = SPLIT ? kSplitCols : a.bn;
+  constexpr uint32_t kABytes = 128u * 128u;
+  const uint32_t stage_bytes = kABytes + (uint32_t)bn * 128u, ring = base + 1024u;  // (the partial tile takes the ring's place)
+  auto full_bar = [&](int s) { return base + 8u * (uint32_t)s; };
+  auto empty_bar = [&](int s) { return base + 8u * (uint32_t)(kMostStages + s); };
+  auto acc_full_bar = [&](int b) { return base + 8u * (uint32_t)(2 * kMostStages + b); };
+  auto acc_empty_bar = [&](int b) { return base + 8u * (uint32_t)(2 * kMostStages + 2 + b); };
+  constexpr int kBars = 2 * kMostStages + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 8 * kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 8 * kBars + 4);
+  if ((int)threadIdx.x < kBars) {
+    mbar_init(base + 8u * threadIdx.x, (int)threadIdx.x >= 2 * kMostStages + 2 ? 4u : 1u);
+    if (threadIdx.x == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), (uint32_t)a.tmem_cols);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&a.a_map);
+    prefetch_tensormap(&a.b_map);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const int per = a.group_m * a.tiles_n, band = tile / per, rest = tile - band * per;
+  const int high = min(a.group_m, a.tiles_m - band * a.group_m), nt = rest / high;
+  const int m0 = (band * a.group_m + rest - nt * high) * 128, n0 = nt * bn;
+  const int k0 = rank * a.blocks_per_split, k1 = min(k0 + a.blocks_per_split, a.kblocks);
+  const int parts = SPLIT ? kParts : 1;
+
+  if (warp == 0) {
+    // ------------------------------- producer ------------------------------------------------
+    grid_dependency_wait();
+    grid_launch_dependents();  // (the columns of tensor memory are taken)
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int kb = k0; kb < k1 && ok; ++kb)
+#pragma unroll 1
+      for (int part = 0; part < parts; ++part) {
+        if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x2100u + (unsigned)s)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = full_bar(s), sa = ring + (uint32_t)s * stage_bytes, sb = sa + kABytes;
+        const int ka = kb * kStepK + (SPLIT ? part_of_a(part) * a.part_k : 0), kc = kb * kStepK + (SPLIT ? part_of_b(part) * a.part_k : 0);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(fb, stage_bytes);
+          if (a.a_mn) {
+            load_2d(sa, &a.a_map, fb, m0, ka);
+            load_2d(sa + 8192u, &a.a_map, fb, m0 + 64, ka);
+          } else {
+            load_2d(sa, &a.a_map, fb, ka, m0);
+          }
+          if (a.b_mn) {
+            load_2d(sb, &a.b_map, fb, n0, kc);
+            if (bn > 64) load_2d(sb + 8192u, &a.b_map, fb, n0 + 64, kc);
+          } else {
+            load_2d(sb, &a.b_map, fb, kc, n0);
+          }
+        }
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+  } else if (warp == 1) {
+    // ------------------------------- MMA issuer -----------------------------------------------
+    const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo);
+    const uint32_t a_kadv = a.a_kadv >> 4, b_kadv = a.b_kadv >> 4, idesc = a.idesc;
+    int s = 0;
+    uint32_t ph = 0, buf = 0, aph = 0, accumulate = 0u;
+    bool ok = true;
+    grid_dependency_wait();
+#pragma unroll 1
+    for (int kb = k0; kb < k1 && ok; ++kb) {
+      if constexpr (SPLIT) {
+        if (!warp_wait(acc_empty_bar((int)buf), aph ^ 1u, abort_flag, a, 0x2200u + buf)) break;
+        tc_fence_after_sync();
+        accumulate = 0u;
+      }
+      const uint32_t d = tmem_base + (SPLIT ? buf * (uint32_t)kSplitCols : 0u);
+#pragma unroll 1
+      for (int part = 0; part < parts; ++part) {
+        if (!warp_wait(full_bar(s), ph, abort_flag, a, 0x2300u + (unsigned)s)) {
+          ok = false;
+          break;
+        }
+        const uint32_t sa = (ring + (uint32_t)s * stage_bytes) & 0x3FFFFu;
+        const uint64_t da = a_desc0 + (uint64_t)(sa >> 4), db = b_desc0 + (uint64_t)((sa + kABytes) >> 4);
+        warp_mma_f16(d, da, db, idesc, accumulate);
+        warp_mma_f16(d, da + a_kadv, db + b_kadv, idesc, 1u);
+        warp_mma_f16(d, da + 2 * a_kadv, db + 2 * b_kadv, idesc, 1u);
+        warp_mma_f16(d, da + 3 * a_kadv, db + 3 * b_kadv, idesc, 1u);
+        accumulate = 1u;
+        warp_commit(empty_bar(s));
+        if (++s == S) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      if constexpr (SPLIT) {
+        if (!ok) break;
+        warp_commit(acc_full_bar((int)buf));
+        if (++buf == 2u) {
+          buf = 0;
+          aph ^= 1u;
+        }
+      }
+    }
+    if (!SPLIT) warp_commit(acc_full_bar(0));
+  }
+  // ------------------------------- partial tile -> shared memory ------------------------------
+  // A line of 16 bytes more than it holds: [row][column], or [column][row] where rows are the result's columns.
+  const uint32_t line = (uint32_t)(a.swapped ? 128 : bn) * 4u + 16u;
+  if (warp >= 2) {
+    grid_dependency_wait();
+    const int q = warp & 3, row = q * 32 + lane;
+    const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
+    auto put = [&](int c0, const float* v) {  // 16 columns
+      if (a.swapped) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<float*>(smem + 1024 + (size_t)(c0 + i) * line + row * 4) = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(smem + 1024 + (size_t)row * line + (c0 + i) * 4) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
+    };
+    if constexpr (SPLIT) {
+      float sums[kSplitCols];
+#pragma unroll
+      for (int i = 0; i < kSplitCols; ++i) sums[i] = 0.f;
+      uint32_t buf = 0, aph = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int kb = k0; kb < k1; ++kb) {
+        if (!warp_wait(acc_full_bar((int)buf), aph, abort_flag, a, 0x2400u + buf)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < kSplitCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32(lanes + buf * (uint32_t)kSplitCols + (uint32_t)c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[c + i] += __uint_as_float(r[i]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty_bar((int)buf));
+        if (++buf == 2u) {
+          buf = 0;
+          aph ^= 1u;
+        }
+      }
+      // (the last accumulator is full: every copy into the ring has landed and every MMA has read it; so for all four warps)
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < kSplitCols; c += 16) put(c, sums + c);
+      }
+    } else {
+      if (warp_wait(acc_full_bar(0), 0u, abort_flag, a, 0x2400u)) {
+        tc_fence_after_sync();
+#pragma unroll 1
+        for (int c = 0; c < bn; c += 16) {
+          uint32_t r[16];
+          tmem_ld_32x16(lanes + (uint32_t)c, r);
+          tmem_wait_ld();
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+          put(c, v);
+        }
+      }
+    }
+    tc_fence_before_sync();
+  }
+  __syncwarp();
+  cluster_sync_all();
+  // ------------------------------- the CTA's share of the result ------------------------------
+  if (!*abort_flag) {
+    const Finish& f = a.f;
+    grid_dependency_wait();
+    const int rows = 128 / splits, quads = a.swapped ? rows / 4 : bn / 4;  // tile rows of this CTA; fours in a line of the result
+    const int lines = a.swapped ? min(bn, f.rows - n0) : min(rows, f.rows - m0 - rank * rows);
+#pragma unroll 2
+    for (int i = (int)threadIdx.x; i < lines * quads; i += kSoloThreads) {
+      const int l = i / quads, c = (i - l * quads) * 4;
+      const long long r = a.swapped ? n0 + l : m0 + rank * rows + l;       // row and first column of the result
+      const int col = a.swapped ? m0 + rank * rows + c : n0 + c, left = f.cols - col;
+      if (left <= 0) continue;
+      const uint32_t at = base + 1024u + (a.swapped ? (uint32_t)l * line + (uint32_t)(rank * rows + c) * 4u
+                                                    : (uint32_t)(rank * rows + l) * line + (uint32_t)c * 4u);
+      float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (f.bias != nullptr) load_four<OutT>(static_cast<const OutT*>(f.bias) + col, a.bias_vec, left, v);
+      if (f.aux != nullptr) load_four<OutT>(static_cast<const OutT*>(f.aux) + r * f.aux_pitch + col, a.aux_vec, left, x);
+      float z[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < splits; ++k) {
+        const float4 p = ld_cluster_v4(cluster_map_shared(at, (uint32_t)k));
+        z[0] += p.x, z[1] += p.y, z[2] += p.z, z[3] += p.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += z[j];
+      if (f.pre != nullptr) store_four<OutT>(static_cast<OutT*>(f.pre) + r * f.pre_pitch + col, a.pre_vec, left, v);
+      with_activation(f.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (f.gradient)
+            v[j] = f.aux != nullptr ? v[j] * slope_of<ACT, OutT>(x[j]) : v[j];
+          else
+            v[j] = f.scale * value_of<ACT, OutT>(v[j]) + x[j];
+        }
+      });
+      store_four<OutT>(static_cast<OutT*>(f.out) + r * f.out_pitch + col, a.out_vec, left, v);
+    }
+  } else {
+    const uint64_t t0 = global_timer_ns();  // copies already issued may still be landing in shared memory
+    while (global_timer_ns() - t0 < 200000ull) {
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();  // no CTA leaves while another may still read its partial tile
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, (uint32_t)a.tmem_cols);
+  }
+}
+
+// ---- fp32 operands in three parts ---------------------------------------------------------------------
+// x = p0 + p1 + p2 + (at most 2^-25 of x): each part the rest rounded to bf16, the rests themselves exact.  to[part][..]: parts are
+// `part_stride` elements apart; rows x cols of the source, zeros up to to_rows x to_cols.
+__global__ void __launch_bounds__(256) split_parts_kernel(const float* from, long long pitch, int rows, int cols, __nv_bfloat16* to,
+                                                          long long to_pitch, long long part_stride, size_t pairs, int to_cols) {
+  overlap_wait();
+  const int half_cols = to_cols / 2;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / half_cols;
+    const int c = (int)(i - r * half_cols) * 2;
+    float v[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = r < (size_t)rows && c + j < cols ? from[(long long)r * pitch + c + j] : 0.f;
+    __nv_bfloat162* at = reinterpret_cast<__nv_bfloat162*>(to + (long long)r * to_pitch + c);
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+      __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
+      if (__hisinf(p.x)) p.x = __float2bfloat16_rz(v[0]);  // (finite values beyond bf16's largest)
+      if (__hisinf(p.y)) p.y = __float2bfloat16_rz(v[1]);
+      *at = p;
+      at += part_stride / 2;
+      v[0] -= __low2float(p);
+      v[1] -= __high2float(p);
+    }
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+// Boxes of 128 bytes x box_rows of a matrix of rows x cols elements, zeros outside it, swizzled.
+bool matrix_map(CUtensorMap* map, int dtype, const void* p, long long pitch, long long rows, long long cols, int box_rows) {
+  const EncodeFn fn = encoder();
+  if (fn == nullptr) {
+    fail(PDNN_ALLOCATION_PROBLEM, "cuTensorMapEncodeTiled is unavailable");
+    return false;
+  }
+  const cuuint64_t es = dtype_size(dtype);
+  if (rows == 1) pitch = (long long)((cols * es + 15) / 16 * 16 / es);  // (no row follows)
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * es};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const CUtensorMapDataType dt = dtype == PDNN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                               : dtype == PDNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = fn(map, dt, 2, const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    fail(PDNN_INVALID_PARAMETER, "cuTensorMapEncodeTiled failed (%d): %lld x %lld, pitch %lld", (int)r, rows, cols, pitch);
+  return r == CUDA_SUCCESS;
+}
+
+bool tma_ok(int dtype, const void* p, long long pitch, int rows) {
+  const long long bytes = pitch * (long long)dtype_size(dtype);
+  return aligned16(p) && (rows == 1 || (bytes % 16 == 0 && bytes < (1ll << 40)));
+}
+bool fours_ok(int dtype, const void* p, long long pitch) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * dtype_size(dtype)) == 0 && pitch % 4 == 0;
+}
+
+// An operand as the kernels see it: `mn` rows or columns of the tile's side, MN-major or K-major.
+struct Side {
+  const void* p;
+  long long pitch;
+  int mn, mn_major;
+};
+
+constexpr int kPairStage256 = 32768, kPairStage128 = 24576;
+
+struct Plan {
+  bool pair;
+  int bn, splits;
+  bool swapped;
+};
+
+// Estimated time in cycles of the plans, from what bounds them: an SM takes a 128 x 256 x 64 step of a pair's tile in 512 cycles; a CTA
+// alone pulls its operands of 16 KB + 128 B a column through L2 at about 40 bytes a cycle while all SMs do, and a step takes
+// it no less than 150 cycles.  A pair's tile ends with about 2500 cycles (the last one's end is not hidden), a CTA's with
+// 2500 and 400 for each partial tile it adds.
+Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_major, int kblocks, int sms) {
+  const double parts = split ? kParts : 1;
+  auto tiles = [](long long x, int t) { return (x + t - 1) / t; };
+  Plan best{true, 128, 1, false};
+  double least = 1e30;
+  for (int bn : {256, 128}) {
+    if (split && bn == 256) continue;
+    const double waves = (double)tiles(tiles(m, 256) * tiles(n, bn), sms / 2);
+    const double t = waves * kblocks * parts * 2.0 * bn + 3500 + (split ? 2000 : 0);
+    if (t < least) least = t, best = Plan{true, bn, 1, false};
+  }
+  for (int swapped = 0; swapped < 2; ++swapped)
+    for (int bn : {16, 32, 64, 128}) {
+      if (split && bn != kSplitCols) continue;
+      if (bn < 64 && (swapped ? m_major : n_major)) continue;  // (an MN-major tile is whole boxes of 64 columns)
+      const long long rows = swapped ? n : m, cols = swapped ? m : n;
+      const long long t1 = tiles(rows, 128) * tiles(cols, bn);
+      if (t1 > 8ll * sms) continue;
+      for (int splits : {1, 2, 4, 8}) {
+        if (splits > 1 && (kblocks + splits - 1) / splits * (splits - 1) >= kblocks) continue;  // a CTA without steps
+        const long long ctas = t1 * splits;
+        const double steps = (double)((kblocks + splits - 1) / splits) * parts;
+        const double step = std::max(150.0, (16384.0 + 128.0 * bn) / 40.0);
+        const double waves = (double)tiles(ctas, sms);
+        const double t = waves * steps * step + (ctas > 2 * sms ? waves / 2 : 1) * (2500 + 400 * splits);
+        if (t < least) least = t, best = Plan{false, bn, splits, swapped != 0};
+      }
+    }
+  return best;
+}
+
+int opt_in(const void* kernel, int bytes) {
+  // once per kernel and device
+  static std::mutex mu;
+  struct Entry {
+    const void* kernel;
+    int dev;
+  };
+  static Entry known[256];
+  static int count = 0;
+  const int dev = current_device();
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < count; ++i)
+    if (known[i].kernel == kernel && known[i].dev == dev) return PDNN_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: cannot opt in to %d bytes of shared memory", bytes);
+  }
+  if (count < 256) known[count++] = Entry{kernel, dev};
+  return PDNN_OK;
+}
+
+int launch_cluster(void (*kernel)(FusedArgs), const FusedArgs& args, unsigned grid, unsigned threads, size_t smem, unsigned cluster,
+                   cudaStream_t s) {
+  const int st = opt_in(reinterpret_cast<const void*>(kernel), kSmemBudget);
+  if (st != PDNN_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: launch failed: %s", cudaGetErrorString(e));
+  }
+  return check_launch("matmul_fused");
+}
+
+// dtype: of the operands (f16 or bf16); out_dtype: of the finish's tensors.
+template <typename OutT, bool SPLIT>
+int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, int part_k, const Finish& f, cudaStream_t s) {
+  const int sms = device_sm_count();
+  FusedArgs a;
+  std::memset(&a, 0, sizeof(a));
+  if (plan.swapped) std::swap(x, y);
+  const int bm = plan.pair ? 256 : 128;
+  a.f = f;
+  a.error_record = tc_error_record_address();
+  if (a.error_record == nullptr) return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: no error record");
+  a.wait_limit_ns = kWaitLimitNs;
+  a.tiles_m = (x.mn + bm - 1) / bm;
+  a.tiles_n = (y.mn + plan.bn - 1) / plan.bn;
+  a.group_m = std::min(a.tiles_m, 8);
+  a.kblocks = (k + kStepK - 1) / kStepK;
+  a.part_k = part_k;
+  a.a_mn = x.mn_major;
+  a.b_mn = y.mn_major;
+  a.a_lbo = x.mn_major ? 8192u : 16u;
+  a.b_lbo = y.mn_major ? 8192u : 16u;
+  a.a_sbo = a.b_sbo = 1024u;
+  a.a_kadv = x.mn_major ? 2048u : 32u;
+  a.b_kadv = y.mn_major ? 2048u : 32u;
+  a.idesc = make_idesc(dtype == PDNN_BF16 ? 1 : 0, x.mn_major, y.mn_major, plan.bn, plan.pair ? 256 : 128);
+  const long long depth = SPLIT ? 3ll * part_k : k;  // elements along K in memory
+  const int b_cols = plan.pair ? plan.bn / 2 : plan.bn;
+  if (!matrix_map(&a.a_map, dtype, x.p, x.pitch, x.mn_major ? depth : x.mn, x.mn_major ? x.mn : depth, x.mn_major ? kStepK : 128) ||
+      !matrix_map(&a.b_map, dtype, y.p, y.pitch, y.mn_major ? depth : y.mn, y.mn_major ? y.mn : depth, y.mn_major ? kStepK : b_cols))
+    return PDNN_INVALID_PARAMETER;
+  if (plan.pair) {
+    a.out_tma = tma_ok(out_dtype, f.out, f.out_pitch, f.rows);
+    a.aux_tma = f.aux != nullptr && tma_ok(out_dtype, f.aux, f.aux_pitch, f.rows);
+    a.pre_tma = f.pre != nullptr && tma_ok(out_dtype, f.pre, f.pre_pitch, f.rows);
+    if ((a.out_tma && !matrix_map(&a.out_map, out_dtype, f.out, f.out_pitch, f.rows, f.cols, 32)) ||
+        (a.aux_tma && !matrix_map(&a.aux_map, out_dtype, f.aux, f.aux_pitch, f.rows, f.cols, 32)) ||
+        (a.pre_tma && !matrix_map(&a.pre_map, out_dtype, f.pre, f.pre_pitch, f.rows, f.cols, 32)))
+      return PDNN_INVALID_PARAMETER;
+    const int stage = plan.bn == 256 ? kPairStage256 : kPairStage128;
+    const int fixed = 1024 + 2 * kEndWarps * kSlotBytes + 8 * (2 * kMostStages + 4 + 2 * kEndWarps) + 16 + kEndWarps * 128;
+    a.stages = std::min(kMostStages, (kSmemBudget - fixed) / stage);
+    const unsigned grid = (unsigned)std::min<long long>(2ll * a.tiles_m * a.tiles_n, sms / 2 * 2);
+    void (*kernel)(FusedArgs) = nullptr;
+    if constexpr (SPLIT)
+      kernel = pair_gemm_kernel<OutT, 128, true>;
+    else
+      kernel = plan.bn == 256 ? pair_gemm_kernel<OutT, 256, false> : pair_gemm_kernel<OutT, 128, false>;
+    tc_set_last_kernel("pair_gemm_kernel");
+    return launch_cluster(kernel, a, grid, kPairThreads, (size_t)fixed + (size_t)a.stages * stage, 2, s);
+  }
+  a.bn = plan.bn;
+  a.splits = plan.splits;
+  a.blocks_per_split = (a.kblocks + plan.splits - 1) / plan.splits;
+  a.swapped = plan.swapped;
+  const int columns = SPLIT ? 2 * kSplitCols : plan.bn;
+  a.tmem_cols = std::max(32, columns);
+  a.out_vec = fours_ok(out_dtype, f.out, f.out_pitch);
+  a.aux_vec = fours_ok(out_dtype, f.aux, f.aux_pitch);
+  a.pre_vec = fours_ok(out_dtype, f.pre, f.pre_pitch);
+  a.bias_vec = fours_ok(out_dtype, f.bias, 0);
+  const int stage = 16384 + plan.bn * 128;
+  a.stages = std::min(kMostStages, (kSoloSmem - kSoloHead) / stage);
+  const size_t partial = plan.swapped ? (size_t)plan.bn * (128 * 4 + 16) : (size_t)128 * (plan.bn * 4 + 16);
+  const size_t smem = kSoloHead + std::max((size_t)a.stages * stage, partial);
+  tc_set_last_kernel("solo_gemm_kernel");
+  void (*kernel)(FusedArgs) = solo_gemm_kernel<OutT, SPLIT>;
+  return launch_cluster(kernel, a, (unsigned)(a.tiles_m * a.tiles_n * plan.splits), kSoloThreads, smem, (unsigned)plan.splits, s);
+}
+
+}  // namespace
+
+bool fused_gemm_operand_ok(int dtype, const Matrix& m) { return dtype == PDNN_F32 || tma_ok(dtype, m.p, m.pitch, m.rows); }
+
+int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, cudaStream_t s) {
+  const int sms = device_sm_count();
+  Side x{a.p, a.pitch, f.rows, ta}, y{b.p, b.pitch, f.cols, !tb};
+  const int kblocks = (k + kStepK - 1) / kStepK;
+  Plan plan = choose_plan(dtype == PDNN_F32, f.rows, f.cols, x.mn_major != 0, y.mn_major != 0, kblocks, sms);
+  if (dtype == PDNN_F16) return run_plan<__half, false>(plan, dtype, dtype, x, y, k, 0, f, s);
+  if (dtype == PDNN_BF16) return run_plan<__nv_bfloat16, false>(plan, dtype, dtype, x, y, k, 0, f, s);
+  // parts behind one another along K
+  const int part_k = kblocks * kStepK;
+  const Matrix* from[2] = {&a, &b};
+  Side* side[2] = {&x, &y};
+  size_t bytes[2], cols[2];
+  for (int i = 0; i < 2; ++i) {
+    cols[i] = side[i]->mn_major ? ((size_t)side[i]->mn + 7) / 8 * 8 : (size_t)part_k;
+    bytes[i] = (side[i]->mn_major ? (size_t)part_k : (size_t)side[i]->mn) * cols[i] * 3 * 2;
+    bytes[i] = (bytes[i] + 255) / 256 * 256;
+  }
+  char* scratch = nullptr;
+  if (cudaMallocAsync(reinterpret_cast<void**>(&scratch), bytes[0] + bytes[1], s) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: cannot allocate %zu bytes of scratch", bytes[0] + bytes[1]);
+  }
+  int st = PDNN_OK;
+  for (int i = 0; i < 2 && st == PDNN_OK; ++i) {
+    __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(scratch + (i == 0 ? 0 : bytes[0]));
+    const size_t rows = side[i]->mn_major ? (size_t)part_k : (size_t)side[i]->mn;
+    const long long pitch = side[i]->mn_major ? (long long)cols[i] : 3ll * part_k;
+    const long long part_stride = side[i]->mn_major ? (long long)part_k * (long long)cols[i] : part_k;
+    const size_t pairs = rows * (cols[i] / 2);
+    launch_overlapped(split_parts_kernel, grid_for(pairs, 256, sms), 256, s, static_cast<const float*>(from[i]->p), from[i]->pitch,
+                      from[i]->rows, from[i]->cols, to, pitch, part_stride, pairs, (int)cols[i]);
+    st = check_launch("matmul_fused: parts");
+    side[i]->p = to;
+    side[i]->pitch = pitch;
+  }
+  if (st == PDNN_OK) st = run_plan<float, true>(plan, PDNN_BF16, PDNN_F32, x, y, k, part_k, f, s);
+  cudaFreeAsync(scratch, s);
+  return st;
+}
+
+}  // namespace pdnn

@@ -3,10 +3,11 @@
 //   z = lhs * rhs + bias,  out = residual + scale * act(z)
 //   dz = scale * dy * act'(z),  d_lhs = dz * rhs^T (times act_in'(z_in)),  d_rhs = lhs^T * dz,  d_bias = sum of dz's rows
 //
-// General form, in two steps: the product in fp32, in scratch, and one pass over it for the rest.
+// Each product with its end is one launch of fused_gemm.cu's.  What is left here is dz - the elementwise slope, one pass that
+// takes the bias gradient's sums on its way - and copies of 16-bit operands that TMA cannot read in place.
 #include "activation.cuh"
 #include "column_sums.cuh"
-#include "tc_gemm.cuh"
+#include "fused_gemm.cuh"
 
 #include <algorithm>
 #include <cstring>
@@ -46,109 +47,40 @@ int dispatch(int dtype, F&& f) {
   return fail(PDNN_INVALID_PARAMETER, "matmul_fused: unknown dtype %d", dtype);
 }
 
-// A matrix in memory: `rows` rows of `cols` elements, `pitch` elements apart.
-struct Matrix {
-  const void* p;
-  long long pitch;
-  int rows, cols;
-};
-
-// rows x cols of the source, zeros up to to_rows x to_cols.
-template <typename W>
-__global__ void __launch_bounds__(256) pad_matrix_kernel(const W* from, long long pitch, int rows, int cols, W* to, size_t items,
-                                                         int to_cols) {
+// The 16-bit elements of a matrix in rows of to_cols, zeros behind the matrix' own.
+__global__ void __launch_bounds__(256) pad_matrix_kernel(const unsigned short* from, long long pitch, int cols, unsigned short* to,
+                                                         size_t items, int to_cols) {
   overlap_wait();
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (size_t)gridDim.x * 256) {
     const size_t r = i / to_cols;
     const int c = (int)(i - r * to_cols);
-    to[i] = r < (size_t)rows && c < cols ? from[(long long)r * pitch + c] : W(0);
+    to[i] = c < cols ? from[(long long)r * pitch + c] : (unsigned short)0;
   }
 }
 
-int pad_matrix(int dtype, const Matrix& a, void* to, int to_rows, int to_cols, cudaStream_t s) {
-  const size_t items = (size_t)to_rows * to_cols;
-  const unsigned grid = grid_for(items, 256, device_sm_count());
-  if (dtype == PDNN_F32)
-    launch_overlapped(pad_matrix_kernel<unsigned>, grid, 256, s, static_cast<const unsigned*>(a.p), a.pitch, a.rows, a.cols,
-                      static_cast<unsigned*>(to), items, to_cols);
-  else
-    launch_overlapped(pad_matrix_kernel<unsigned short>, grid, 256, s, static_cast<const unsigned short*>(a.p), a.pitch, a.rows,
-                      a.cols, static_cast<unsigned short*>(to), items, to_cols);
-  return check_launch("matmul_fused: padding");
-}
-
-// What is made of a product.
-struct Finish {
-  const void* bias;
-  const void* aux;     // forward: the residual; gradient: what the slope is taken of
-  void* pre;           // forward: z
-  void* out;
-  long long aux_pitch, pre_pitch, out_pitch;
-  int rows, cols, act, gradient;
-  float scale;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) finish_product_kernel(const float* z, long long z_pitch, const Finish f) {
-  overlap_wait();
-  const size_t items = (size_t)f.rows * f.cols;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (size_t)gridDim.x * 256) {
-    const long long r = (long long)(i / f.cols);
-    const int c = (int)(i - (size_t)r * f.cols);
-    float v = z[r * z_pitch + c];
-    if (f.bias != nullptr) v += to_f32(static_cast<const T*>(f.bias)[c]);
-    if (f.pre != nullptr) static_cast<T*>(f.pre)[r * f.pre_pitch + c] = from_f32<T>(v);
-    if (f.gradient) {
-      if (f.aux != nullptr) v *= activation_slope(f.act, to_f32(static_cast<const T*>(f.aux)[r * f.aux_pitch + c]));
-    } else {
-      v = f.scale * activate(f.act, v);
-      if (f.aux != nullptr) v += to_f32(static_cast<const T*>(f.aux)[r * f.aux_pitch + c]);
-    }
-    static_cast<T*>(f.out)[r * f.out_pitch + c] = from_f32<T>(v);
-  }
-}
-
-// op(a) [m][k] times op(b) [k][n], ta / tb: stored the other way round, with f's finish.
-int product(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int m, int k, int n, const Finish& f, cudaStream_t s) {
-  const size_t es = dtype_size(dtype), unit = 16 / es;
-  // The engine takes dense operands whose rows are whole 16-byte packets.
-  const int pm = ta ? (int)round_up(m, unit) : m, pn = (int)round_up(n, unit);
-  const int pk = !ta || tb ? (int)round_up(k, unit) : k;
-  struct {
-    const Matrix* m;
-    int rows, cols;
-    const void* p;
-    size_t bytes;
-  } op[2] = {{&a, ta ? pk : pm, ta ? pm : pk, a.p, 0}, {&b, tb ? pn : pk, tb ? pk : pn, b.p, 0}};
-  size_t need = round_up((size_t)pm * pn * sizeof(float), 256);
-  for (auto& o : op) {
-    if (o.m->rows != o.rows || o.m->cols != o.cols || (o.m->pitch != o.m->cols && o.m->rows > 1) || !aligned16(o.p))
-      o.bytes = round_up((size_t)o.rows * o.cols * es, 256);
-    need += o.bytes;
-  }
+// op(a) times op(b) with f's finish; ta, tb: stored the other way round.
+int product(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, cudaStream_t s) {
+  Matrix in[2] = {a, b};
+  size_t bytes[2] = {0, 0};
+  const size_t es = dtype_size(dtype);
+  for (int i = 0; i < 2; ++i)
+    if (!fused_gemm_operand_ok(dtype, in[i])) bytes[i] = round_up((size_t)in[i].rows * round_up(in[i].cols, 16 / es) * es, 256);
   Scratch scratch(s);
-  if (!scratch.get(need)) return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: cannot allocate %zu bytes of scratch", need);
-  char* at = static_cast<char*>(scratch.p);
-  float* z = reinterpret_cast<float*>(at);
-  at += round_up((size_t)pm * pn * sizeof(float), 256);
-  for (auto& o : op) {
-    if (o.bytes == 0) continue;
-    const int st = pad_matrix(dtype, *o.m, at, o.rows, o.cols, s);
+  if (!scratch.get(bytes[0] + bytes[1]))
+    return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: cannot allocate %zu bytes of scratch", bytes[0] + bytes[1]);
+  for (int i = 0; i < 2; ++i) {
+    if (bytes[i] == 0) continue;
+    char* to = static_cast<char*>(scratch.p) + (i == 0 ? 0 : bytes[0]);
+    const int pitch = (int)round_up(in[i].cols, 16 / es);
+    const size_t items = (size_t)in[i].rows * pitch;
+    launch_overlapped(pad_matrix_kernel, grid_for(items, 256, device_sm_count()), 256, s, static_cast<const unsigned short*>(in[i].p),
+                      in[i].pitch, in[i].cols, reinterpret_cast<unsigned short*>(to), items, pitch);
+    const int st = check_launch("matmul_fused: padding");
     if (st != PDNN_OK) return st;
-    o.p = at;
-    at += o.bytes;
+    in[i].p = to;
+    in[i].pitch = pitch;
   }
-  int st;
-  if (tc_matmul_supported(dtype, ta, tb, op[0].p, op[1].p, z, 1, pm, pk, pn))
-    st = tc_matmul(dtype, ta, tb, op[0].p, op[1].p, z, 1, pm, pk, pn, 0.f, s, /*out_f32=*/true);
-  else
-    st = simt_matmul(dtype, ta, tb, op[0].p, op[1].p, z, 1, pm, pk, pn, 0.f, s, /*out_f32=*/true);
-  if (st != PDNN_OK) return st;
-  const unsigned grid = grid_for((size_t)f.rows * f.cols, 256, device_sm_count());
-  return dispatch(dtype, [&](auto type) {
-    launch_overlapped(finish_product_kernel<decltype(type)>, grid, 256, s, z, (long long)pn, f);
-    return check_launch("matmul_fused: epilogue");
-  });
+  return fused_gemm(dtype, ta, tb, in[0], in[1], k, f, s);
 }
 
 // ---- dz and the bias gradient -----------------------------------------------------------------------
@@ -272,7 +204,7 @@ int launch_matmul_fused(int dtype, const void* lhs, const void* rhs, void* out, 
   f.act = e.activation;
   f.scale = e.scale;
   const Matrix a{lhs, p.lhs_pitch, p.m, p.k}, b{rhs, p.rhs_pitch, p.transpose_rhs ? p.n : p.k, p.transpose_rhs ? p.k : p.n};
-  return product(dtype, 0, p.transpose_rhs, a, b, p.m, p.k, p.n, f, s);
+  return product(dtype, 0, p.transpose_rhs, a, b, p.k, f, s);
 }
 
 int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, const void* rhs, const PdnnMatmulParams& p,
@@ -309,7 +241,7 @@ int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, c
     f.gradient = 1;
     f.aux = g.input_activation != PDNN_ACT_NONE ? g.input_pre_activation : nullptr;
     f.aux_pitch = g.input_pre_activation_pitch;
-    const int st = product(dtype, 0, !p.transpose_rhs, dz, Matrix{rhs, p.rhs_pitch, w_rows, w_cols}, p.m, p.n, p.k, f, s);
+    const int st = product(dtype, 0, !p.transpose_rhs, dz, Matrix{rhs, p.rhs_pitch, w_rows, w_cols}, p.n, f, s);
     if (st != PDNN_OK) return st;
   }
   if (g.rhs_grad != nullptr) {
@@ -318,9 +250,10 @@ int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, c
     f.out_pitch = g.rhs_grad_pitch;
     f.rows = w_rows;
     f.cols = w_cols;
+    f.act = PDNN_ACT_NONE;
     f.gradient = 1;
     const Matrix x{lhs, p.lhs_pitch, p.m, p.k};
-    const int st = p.transpose_rhs ? product(dtype, 1, 0, dz, x, p.n, p.m, p.k, f, s) : product(dtype, 1, 0, x, dz, p.k, p.m, p.n, f, s);
+    const int st = p.transpose_rhs ? product(dtype, 1, 0, dz, x, p.m, f, s) : product(dtype, 1, 0, x, dz, p.m, f, s);
     if (st != PDNN_OK) return st;
   }
   return PDNN_OK;

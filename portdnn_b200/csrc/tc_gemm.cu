@@ -4521,6 +4521,7 @@ int simt_matmul(int dtype, int tl, int tr, const void* lhs, const void* rhs, voi
 }
 
 const char* tc_last_kernel() { return t_last_kernel; }
+void tc_set_last_kernel(const char* name) { t_last_kernel = name; }
 
 bool tc_dense_nhwc_map(CUtensorMap* map, int dtype, const void* base, int n, int h, int w, int c, const uint32_t box[4]) {
   const uint64_t es = dtype_size(dtype);

@@ -45,6 +45,7 @@ int simt_matmul(int dtype, int tl, int tr, const void* lhs, const void* rhs, voi
 
 // Name of the tensor-core kernel that the calling thread launched last ("" before the first).
 const char* tc_last_kernel();
+void tc_set_last_kernel(const char* name);  // (a literal; for kernels outside tc_gemm.cu)
 
 // Tensor map of a dense NHWC tensor whose box lands in shared memory as it is (no swizzle), zeros outside the tensor.
 // False, with the error text set, where it cannot be encoded.
