@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libportdnn_b200.so")
 FRONT_SOURCE = os.path.join(CSRC, "front.cpp")
 SOURCES = ["c_api.cu", "hbm_kernels.cu", "direct_conv.cu", "tc_gemm.cu", "winograd.cu", "norm_kernels.cu",
            "layout_kernels.cu", "padded_conv.cu", "depthwise_tile.cu", "simt_gemm.cu", "collective.cu",
-           "fused_gemm.cu", "fused_matmul.cu", "residual_norm.cu", "policy_loss.cu"]
+           "fused_gemm.cu", "fused_rows.cu", "fused_matmul.cu", "residual_norm.cu", "policy_loss.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"]
 

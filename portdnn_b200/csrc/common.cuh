@@ -78,6 +78,24 @@ __device__ __forceinline__ void store16(T* p, const Vec16<T>& v) {
   *reinterpret_cast<uint4*>(p) = v.raw;
 }
 
+// V elements as a thread keeps them: a 16-byte packet or a single element.
+template <typename T, int V>
+struct Piece {
+  Vec16<T> raw;
+  __device__ __forceinline__ void load(const T* p) { raw = load16(p); }
+  __device__ __forceinline__ float get(int i) const { return to_f32(raw.get(i)); }
+  __device__ __forceinline__ void set(int i, float v) { raw.set(i, from_f32<T>(v)); }
+  __device__ __forceinline__ void store(T* p) const { store16(p, raw); }
+};
+template <typename T>
+struct Piece<T, 1> {
+  T raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *p; }
+  __device__ __forceinline__ float get(int) const { return to_f32(raw); }
+  __device__ __forceinline__ void set(int, float v) { raw = from_f32<T>(v); }
+  __device__ __forceinline__ void store(T* p) const { *p = raw; }
+};
+
 __device__ __forceinline__ float apply_activation(float v, int act) {
   switch (act) {
     case PDNN_ACT_RELU: return fmaxf(v, 0.f);

@@ -27,11 +27,15 @@ namespace {
 
 using namespace umma;
 
-constexpr int kStepK = 64;         // reduction elements of a stage: a 128-byte row of 16-bit elements
+// Reduction elements of a stage: a 128-byte row of 16-bit elements; of an fp32 operand's parts, three times as many bytes, half
+// of that (two stages of 72 KB leave a pair waiting for its copies: 1.9 us to 64 elements, four of 36 KB: kept busy).
+constexpr int step_k(bool split) { return split ? 32 : 64; }
+constexpr int kChainSteps = 2;     // fp32: stages whose products the accumulator takes before it is emptied
 constexpr int kMostStages = 12;
 constexpr int kSlotBytes = 4096;   // 32 rows of 128 bytes, swizzled as TMA does
 constexpr int kSmemBudget = 232448;
-constexpr int kParts = 6;          // products of parts that make an fp32 product
+constexpr int kFewRows = 16;       // fp32 rows that go to fused_rows.cu
+constexpr int kProducts = 6;       // products of parts that make an fp32 product
 
 struct alignas(64) FusedArgs {
   CUtensorMap a_map, b_map, out_map, aux_map, pre_map;
@@ -41,11 +45,11 @@ struct alignas(64) FusedArgs {
   int tiles_m, tiles_n, group_m;     // tiles; rows of tiles that are walked together
   int kblocks, part_k;               // steps along K (of each product of parts); distance between two parts along K
   int a_mn, b_mn, stages;
-  unsigned a_lbo, a_sbo, a_kadv, b_lbo, b_sbo, b_kadv, idesc;
+  unsigned a_lbo, a_sbo, a_layout, a_kadv, b_lbo, b_sbo, b_layout, b_kadv, idesc;
   int out_tma, aux_tma, pre_tma;
   // solo_gemm_kernel
   int bn, splits, blocks_per_split, swapped, tmem_cols;
-  int out_vec, aux_vec, pre_vec, bias_vec;  // four elements at a time
+  int out_vec, aux_vec, pre_vec, bias_vec;  // whole packets at a time
 };
 
 __device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
@@ -69,58 +73,18 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, a.error_record, a.wait_limit_ns, where));
 }
 
-// The product of parts that step `part` takes: first the largest.
-__device__ __forceinline__ int part_of_a(int part) { return part == 2 || part == 3 ? 1 : part == 5 ? 2 : 0; }
-__device__ __forceinline__ int part_of_b(int part) { return part == 1 || part == 3 ? 1 : part == 4 ? 2 : 0; }
+// Which parts the i-th product of a step takes, the smallest products first (16-bit operands have one part and one product).
+template <bool SPLIT>
+__device__ __forceinline__ constexpr int part_of_a(int i) {
+  return !SPLIT || i == 1 || i == 3 || i == 5 ? 0 : i == 0 ? 2 : 1;  // 2 0, 0 2, 1 1, 0 1, 1 0, 0 0
+}
+template <bool SPLIT>
+__device__ __forceinline__ constexpr int part_of_b(int i) {
+  return !SPLIT || i == 0 || i == 4 || i == 5 ? 0 : i == 1 ? 2 : 1;
+}
 
 // Where element byte `b` of row `r` of a slot is.
 __device__ __forceinline__ uint32_t slot_at(int r, int b) { return (uint32_t)(r * 128 + ((((b >> 4) ^ (r & 7)) << 4) | (b & 15))); }
-
-// Phi(z), the normal distribution's function: a polynomial in 1 / (1 + p |x|) times exp(-x^2), x = z / sqrt(2) (Abramowitz and
-// Stegun, 7.1.26; off by 7.5e-8 at most, in the tail relative to exp(-x^2)).  For results of 16 bits.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678f;
-  const float t = __fdividef(1.f, 1.f + 0.3275911f * x);
-  e = __expf(-x * x);
-  const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  return z >= 0.f ? 1.f - q : q;
-}
-
-// The activation ACT, and its slope, for a result of type OutT.
-template <int ACT, typename OutT>
-__device__ __forceinline__ float value_of(float z) {
-  if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_GELU) {
-    float e;
-    return z * normal_cdf(z, e);
-  } else if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_SILU) {
-    return __fdividef(z, 1.f + __expf(-z));
-  } else {
-    return activate(ACT, z);
-  }
-}
-template <int ACT, typename OutT>
-__device__ __forceinline__ float slope_of(float z) {
-  if constexpr (sizeof(OutT) == 2 && ACT == PDNN_ACT_GELU) {
-    float e;
-    const float c = normal_cdf(z, e);
-    return c + z * 0.39894228f * e;
-  } else {
-    return activation_slope(ACT, z);
-  }
-}
-
-template <typename F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
-  switch (act) {
-    case PDNN_ACT_RELU: f(std::integral_constant<int, PDNN_ACT_RELU>{}); break;
-    case PDNN_ACT_TANH: f(std::integral_constant<int, PDNN_ACT_TANH>{}); break;
-    case PDNN_ACT_RELU6: f(std::integral_constant<int, PDNN_ACT_RELU6>{}); break;
-    case PDNN_ACT_GELU: f(std::integral_constant<int, PDNN_ACT_GELU>{}); break;
-    case PDNN_ACT_SILU: f(std::integral_constant<int, PDNN_ACT_SILU>{}); break;
-    case PDNN_ACT_SIGMOID: f(std::integral_constant<int, PDNN_ACT_SIGMOID>{}); break;
-    default: f(std::integral_constant<int, PDNN_ACT_NONE>{}); break;
-  }
-}
 
 // A 16-byte chunk of a slot as floats, and back.
 template <typename OutT>
@@ -188,7 +152,10 @@ template <typename OutT, int BN, bool SPLIT>
 __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid_constant__ FusedArgs args) {
   extern __shared__ uint8_t smem_raw[];
   const FusedArgs& a = args;
-  constexpr uint32_t kABytes = 128u * 128u, kBBytes = (uint32_t)(BN / 2) * 128u, kStage = kABytes + kBBytes;
+  constexpr int kParts = SPLIT ? 3 : 1;  // of an operand in a stage
+  constexpr int kStepK = step_k(SPLIT), kMmas = kStepK / 16;
+  constexpr uint32_t kABytes = 128u * kStepK * 2u, kBBytes = (uint32_t)(BN / 2) * kStepK * 2u, kStage = kParts * (kABytes + kBBytes);
+  constexpr uint32_t kBox = kStepK * 128u;  // 64 columns of an MN-major operand
   constexpr int CB = 128 / (int)sizeof(OutT), kCols = BN / 2, kBlocks = kCols / CB;  // columns of a block, of a warp; blocks of a warp
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
@@ -234,7 +201,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     m0 = (band * a.group_m + rest - nt * high) * 256 + (int)rank * 128;
     n0 = nt * BN;
   };
-  const int parts = SPLIT ? kParts : 1;
 
   if (warp == 0) {
     // ------------------------------- producer ------------------------------------------------
@@ -248,45 +214,48 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
       tile_at(tile, m0, n0);
       n0 += (int)rank * (BN / 2);
 #pragma unroll 1
-      for (int kb = 0; kb < a.kblocks && ok; ++kb)
-#pragma unroll 1
-        for (int part = 0; part < parts; ++part) {
-          if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x1100u + (unsigned)s)) {
-            ok = false;
-            break;
-          }
-          const uint32_t fb = full_bar(s), sa = base + (uint32_t)s * kStage, sb = sa + kABytes;
-          const int ka = kb * kStepK + (SPLIT ? part_of_a(part) * a.part_k : 0), kc = kb * kStepK + (SPLIT ? part_of_b(part) * a.part_k : 0);
-          if (elect_one()) {
-            if (leader) mbar_arrive_expect_tx(fb, 2u * kStage);  // the bytes of both CTAs
+      for (int kb = 0; kb < a.kblocks; ++kb) {
+        if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x1100u + (unsigned)s)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = full_bar(s);
+        if (elect_one()) {
+          if (leader) mbar_arrive_expect_tx(fb, 2u * kStage);  // the bytes of both CTAs
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const uint32_t sa = base + (uint32_t)s * kStage + (uint32_t)part * kABytes;
+            const uint32_t sb = base + (uint32_t)s * kStage + kParts * kABytes + (uint32_t)part * kBBytes;
+            const int k = kb * kStepK + part * a.part_k;
             if (a.a_mn) {
-              load_2d_pair(sa, &a.a_map, fb, m0, ka);
-              load_2d_pair(sa + 8192u, &a.a_map, fb, m0 + 64, ka);
+              load_2d_pair(sa, &a.a_map, fb, m0, k);
+              load_2d_pair(sa + kBox, &a.a_map, fb, m0 + 64, k);
             } else {
-              load_2d_pair(sa, &a.a_map, fb, ka, m0);
+              load_2d_pair(sa, &a.a_map, fb, k, m0);
             }
             if (a.b_mn) {
-              load_2d_pair(sb, &a.b_map, fb, n0, kc);
-              if (BN == 256) load_2d_pair(sb + 8192u, &a.b_map, fb, n0 + 64, kc);
+              load_2d_pair(sb, &a.b_map, fb, n0, k);
+              if (BN == 256) load_2d_pair(sb + kBox, &a.b_map, fb, n0 + 64, k);
             } else {
-              load_2d_pair(sb, &a.b_map, fb, kc, n0);
+              load_2d_pair(sb, &a.b_map, fb, k, n0);
             }
           }
-          __syncwarp();
-          if (++s == S) {
-            s = 0;
-            ph ^= 1u;
-          }
         }
+        __syncwarp();
+        if (++s == S) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer (rank 0) --------------------------------------
     grid_dependency_wait();
     grid_launch_dependents();  // the grid is a single wave, and its columns of tensor memory are taken
     if (leader) {
-      const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo);
+      const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo, a.a_layout), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo, a.b_layout);
       const uint32_t a_kadv = a.a_kadv >> 4, b_kadv = a.b_kadv >> 4, idesc = a.idesc;
-      const int chains = SPLIT ? a.kblocks : 1, steps = SPLIT ? kParts : a.kblocks;  // accumulator fills of a tile, steps of each
+      const int chains = SPLIT ? (a.kblocks + kChainSteps - 1) / kChainSteps : 1;  // accumulator fills of a tile
       int s = 0;
       uint32_t ph = 0, buf = 0, aph = 0;
       bool ok = true;
@@ -300,6 +269,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
           }
           tc_fence_after_sync();
           const uint32_t d = tmem_base + buf * (uint32_t)BN;
+          const int steps = SPLIT ? min(kChainSteps, a.kblocks - chain * kChainSteps) : a.kblocks;
           uint32_t accumulate = 0u;
 #pragma unroll 1
           for (int ks = 0; ks < steps; ++ks) {
@@ -308,12 +278,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
               break;
             }
             const uint32_t sa = (base + (uint32_t)s * kStage) & 0x3FFFFu;  // offset inside the CTA's shared memory
-            const uint64_t da = a_desc0 + (uint64_t)(sa >> 4), db = b_desc0 + (uint64_t)((sa + kABytes) >> 4);
-            warp_mma_f16_pair(d, da, db, idesc, accumulate);
-            warp_mma_f16_pair(d, da + a_kadv, db + b_kadv, idesc, 1u);
-            warp_mma_f16_pair(d, da + 2 * a_kadv, db + 2 * b_kadv, idesc, 1u);
-            warp_mma_f16_pair(d, da + 3 * a_kadv, db + 3 * b_kadv, idesc, 1u);
-            accumulate = 1u;
+            const uint64_t da0 = a_desc0 + (uint64_t)(sa >> 4), db0 = b_desc0 + (uint64_t)((sa + kParts * kABytes) >> 4);
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? kProducts : 1); ++i) {
+              const uint64_t da = da0 + (uint64_t)(part_of_a<SPLIT>(i) * (kABytes >> 4)), db = db0 + (uint64_t)(part_of_b<SPLIT>(i) * (kBBytes >> 4));
+#pragma unroll
+              for (uint32_t k = 0; k < kMmas; ++k) {
+                warp_mma_f16_pair(d, da + k * a_kadv, db + k * b_kadv, idesc, accumulate);
+                accumulate = 1u;
+              }
+            }
             warp_commit_pair(empty_bar(s), cluster_map_shared(empty_bar(s), 1u));  // both CTAs may refill the stage
             if (++s == S) {
               s = 0;
@@ -377,7 +351,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < kCols; ++i) sums[i] = 0.f;
 #pragma unroll 1
-        for (int chain = 0; chain < a.kblocks; ++chain) {
+        for (int chain = 0; chain < a.kblocks; chain += kChainSteps) {
           if (!warp_wait(acc_full_bar((int)buf), aph, abort_flag, a, 0x1400u + buf)) {
             ok = false;
             break;
@@ -410,42 +384,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
       for (int block = 0; block < kBlocks; ++block) {
         const int col = col0 + block * CB, slot = slot_of(block);
         const bool inside = col < f.cols && rows_left > 0;
-        float v[CB];
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b)  // (registers are not indexed at run time)
-            if (b == block) {
-#pragma unroll
-              for (int i = 0; i < CB; ++i) v[i] = sums[b * CB + i];
-            }
-        } else {
-          uint32_t r[CB / 32][32];
-#pragma unroll
-          for (int c = 0; c < CB / 32; ++c) tmem_ld_32x32(acc + (uint32_t)(block * CB + c * 32), r[c]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < CB; ++i) v[i] = __uint_as_float(r[i / 32][i % 32]);
-          if (block + 1 == kBlocks) {  // the accumulator is free
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty_bar((int)buf) & kPeerBitMask);
-          }
-        }
         if (f.bias != nullptr) {
           __syncwarp();
           strip[lane] = from_f32<OutT>(bias[0]);
           if (CB > 32) strip[lane + 32] = from_f32<OutT>(bias[1]);
           __syncwarp();
-#pragma unroll
-          for (int c = 0; c < CB; c += Vec16<OutT>::N) {
-            float b[Vec16<OutT>::N];
-            unpack<OutT>(*reinterpret_cast<const uint4*>(strip + c), b);
-#pragma unroll
-            for (int i = 0; i < Vec16<OutT>::N; ++i) v[c + i] += b[i];
-          }
         }
         if (block + 1 < kBlocks) bias_at(block + 1, bias);
-        uint8_t* my_row = slots + slot * kSlotBytes + lane * 128;
+        uint8_t *my_row = slots + slot * kSlotBytes + lane * 128, *pre_row = slots + kSlotBytes + lane * 128;
         if (has_aux && inside) {
           if (a.aux_tma) {
             if (!warp_wait(aux_bar(w, slot), (aux_phase >> slot) & 1u, abort_flag, a, 0x1500u + (unsigned)slot)) {
@@ -461,33 +407,87 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
         if (lane == 0 && !has_pre) bulk_wait_group_read<0>();
         __syncwarp();
         if (block + 1 < kBlocks && !has_pre) request_aux(block + 1);
-        if (inside) {
-          if (has_pre) {
-            uint8_t* pre_row = slots + kSlotBytes + lane * 128;
+        // Sixteen columns at a time, in a loop that is not unrolled: eight warps that are nowhere near one another in a long
+        // stretch of code wait for instructions.  The next ones are on their way from tensor memory meanwhile.
+        uint32_t next[SPLIT ? 1 : 16];
+        if constexpr (!SPLIT) {
+          tmem_ld_32x16(acc + (uint32_t)(block * CB), next);
+          tmem_wait_ld();
+        }
+#pragma unroll 1
+        for (int c = 0; c < CB; c += 16) {
+          constexpr int N = Vec16<OutT>::N;
+          float v[16];
+          if constexpr (SPLIT) {
+            const int from = (block * CB + c) / 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(pre_row + ((j ^ (lane & 7)) << 4)) = pack<OutT>(v + j * Vec16<OutT>::N);
-          }
-          with_activation(f.act, [&](auto act) {
-            constexpr int ACT = decltype(act)::value, N = Vec16<OutT>::N;
+            for (int i = 0; i < 16; ++i) {  // (registers are not indexed at run time)
+              v[i] = sums[i];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint4* at = reinterpret_cast<uint4*>(my_row + ((j ^ (lane & 7)) << 4));
-              float x[N];
-              if (has_aux) unpack<OutT>(*at, x);
-#pragma unroll
-              for (int i = 0; i < N; ++i) {
-                float& o = v[j * N + i];
-                if (f.gradient) {
-                  if (has_aux) o *= slope_of<ACT, OutT>(x[i]);
-                } else {
-                  o = f.scale * value_of<ACT, OutT>(o);
-                  if (has_aux) o += x[i];
-                }
-              }
-              *at = pack<OutT>(v + j * N);
+              for (int k = 1; k < kCols / 16; ++k) v[i] = from == k ? sums[k * 16 + i] : v[i];
             }
-          });
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(next[i]);
+            if (c + 16 < CB) {
+              tmem_ld_32x16(acc + (uint32_t)(block * CB + c + 16), next);
+            } else if (block + 1 == kBlocks) {  // the accumulator is free
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty_bar((int)buf) & kPeerBitMask);
+            }
+          }
+          if (f.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 16; j += N) {
+              float b[N];
+              unpack<OutT>(*reinterpret_cast<const uint4*>(strip + c + j), b);
+#pragma unroll
+              for (int i = 0; i < N; ++i) v[j + i] += b[i];
+            }
+          }
+          if (inside) {
+            const int chunk = c / N;
+            if (has_pre) {
+#pragma unroll
+              for (int j = 0; j < 16 / N; ++j)
+                *reinterpret_cast<uint4*>(pre_row + (((chunk + j) ^ (lane & 7)) << 4)) = pack<OutT>(v + j * N);
+            }
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+            if (has_aux) {
+#pragma unroll
+              for (int j = 0; j < 16 / N; ++j)
+                unpack<OutT>(*reinterpret_cast<const uint4*>(my_row + (((chunk + j) ^ (lane & 7)) << 4)), x + j * N);
+            }
+            // (one body to a direction and activation, without branches inside: sixteen chains of latencies side by side)
+            if (f.gradient) {
+              with_activation(f.act, [&](auto act) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 s = slope_of<decltype(act)::value, OutT>(make_float2(x[i], x[i + 1]));
+                  v[i] *= f.scale * s.x;
+                  v[i + 1] *= f.scale * s.y;
+                }
+              });
+            } else {
+              with_activation(f.act, [&](auto act) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 o = value_of<decltype(act)::value, OutT>(make_float2(v[i], v[i + 1]));
+                  v[i] = f.scale * o.x + x[i];
+                  v[i + 1] = f.scale * o.y + x[i + 1];
+                }
+              });
+            }
+#pragma unroll
+            for (int j = 0; j < 16 / N; ++j)
+              *reinterpret_cast<uint4*>(my_row + (((chunk + j) ^ (lane & 7)) << 4)) = pack<OutT>(v + j * N);
+          }
+          if constexpr (!SPLIT) tmem_wait_ld();
+        }
+        if (inside) {
           fence_proxy_async_smem();
           __syncwarp();
           if (has_pre) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
 // ------------------------------------------------------------------------------------------------
 // One tile of 128 x bn to a cluster of `splits` CTAs, each of which takes a share of the steps along K.  Partial tiles go to
 // shared memory, where each CTA of the cluster adds up its share of the tile's rows in the order of the ranks and finishes
-// them, four neighbouring elements to a thread.  swapped: the tile's rows are the columns of the result.  Two CTAs fit
+// them, a packet to a thread.  swapped: the tile's rows are the columns of the result.  Two CTAs fit
 // an SM, so that the end of one overlaps the loads of another.
 // ------------------------------------------------------------------------------------------------
 constexpr int kSoloThreads = 192, kSoloSmem = 110 * 1024, kSoloHead = 2048, kSplitCols = 64;
@@ -552,40 +552,107 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   return v;
 }
 
-// Four neighbouring elements of a row, `left` of them inside it.
+__device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// A packet of a row, `left` elements of which are inside it.
 template <typename OutT>
-__device__ __forceinline__ void load_four(const OutT* p, bool vec, int left, float (&v)[4]) {
-  if (vec && left >= 4) {
-    if constexpr (sizeof(OutT) == 4) {
-      const float4 q = *reinterpret_cast<const float4*>(p);
-      v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-    } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(p);
-      const OutT* e = reinterpret_cast<const OutT*>(&q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
-    }
+__device__ __forceinline__ void load_packet(const OutT* p, bool vec, int left, float (&v)[Vec16<OutT>::N]) {
+  constexpr int N = Vec16<OutT>::N;
+  if (vec && left >= N) {
+    unpack<OutT>(*reinterpret_cast<const uint4*>(p), v);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+    for (int i = 0; i < N; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
   }
 }
 template <typename OutT>
-__device__ __forceinline__ void store_four(OutT* p, bool vec, int left, const float (&v)[4]) {
-  if (vec && left >= 4) {
-    if constexpr (sizeof(OutT) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      uint2 q;
-      OutT* e = reinterpret_cast<OutT*>(&q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = from_f32<OutT>(v[i]);
-      *reinterpret_cast<uint2*>(p) = q;
-    }
+__device__ __forceinline__ void store_packet(OutT* p, bool vec, int left, const float (&v)[Vec16<OutT>::N]) {
+  constexpr int N = Vec16<OutT>::N;
+  if (vec && left >= N) {
+    *reinterpret_cast<uint4*>(p) = pack<OutT>(v);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
       if (i < left) p[i] = from_f32<OutT>(v[i]);
+  }
+}
+
+// A CTA's share of the result: it adds up the ranks' partial tiles in their order and finishes what comes of it, a packet to a
+// thread, two packets at a time.
+template <typename OutT, int SPLITS>
+__device__ __forceinline__ void finish_share(const FusedArgs& a, uint32_t partial, uint32_t line, int m0, int n0, int bn, int rank) {
+  constexpr int N = Vec16<OutT>::N, rows = 128 / SPLITS;
+  const Finish& f = a.f;
+  const int shift = __ffs((a.swapped ? rows : bn) / N) - 1;  // packets in a line of the result, a power of two
+  const int lines = a.swapped ? min(bn, f.rows - n0) : min(rows, f.rows - m0 - rank * rows);
+  const int items = lines << shift;
+  for (int i0 = (int)threadIdx.x; i0 < items; i0 += 2 * kSoloThreads) {
+    float z[2][N];
+    float4 got[2][SPLITS][N / 4];
+    long long r[2];
+    int col[2], left[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = i0 + u * kSoloThreads, l = i >> shift, c = (i - (l << shift)) * N;
+      r[u] = a.swapped ? n0 + l : m0 + rank * rows + l;
+      col[u] = a.swapped ? m0 + rank * rows + c : n0 + c;
+      left[u] = i < items ? f.cols - col[u] : 0;
+      if (left[u] <= 0) continue;
+      const uint32_t at = partial + (a.swapped ? (uint32_t)l * line + (uint32_t)(rank * rows + c) * 4u
+                                               : (uint32_t)(rank * rows + l) * line + (uint32_t)c * 4u);
+#pragma unroll
+      for (int k = 0; k < SPLITS; ++k) {
+        const uint32_t from = SPLITS == 1 ? at : cluster_map_shared(at, (uint32_t)k);
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) got[u][k][j] = SPLITS == 1 ? ld_shared_v4(from + 16u * j) : ld_cluster_v4(from + 16u * j);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (left[u] <= 0) continue;
+      float x[N], b[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = b[j] = 0.f;
+      if (f.bias != nullptr) load_packet<OutT>(static_cast<const OutT*>(f.bias) + col[u], a.bias_vec, left[u], b);
+      if (f.aux != nullptr) load_packet<OutT>(static_cast<const OutT*>(f.aux) + r[u] * f.aux_pitch + col[u], a.aux_vec, left[u], x);
+#pragma unroll
+      for (int j = 0; j < N / 4; ++j) {
+        float4 s = got[u][0][j];
+#pragma unroll
+        for (int k = 1; k < SPLITS; ++k) {
+          const float4 p = got[u][k][j];
+          s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
+        }
+        z[u][4 * j] = s.x, z[u][4 * j + 1] = s.y, z[u][4 * j + 2] = s.z, z[u][4 * j + 3] = s.w;
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) z[u][j] += b[j];
+      if (f.pre != nullptr) store_packet<OutT>(static_cast<OutT*>(f.pre) + r[u] * f.pre_pitch + col[u], a.pre_vec, left[u], z[u]);
+      if (f.gradient) {
+        with_activation(f.act, [&](auto act) {
+#pragma unroll
+          for (int j = 0; j < N; j += 2) {
+            const float2 s = slope_of<decltype(act)::value, OutT>(make_float2(x[j], x[j + 1]));
+            z[u][j] *= f.scale * s.x;
+            z[u][j + 1] *= f.scale * s.y;
+          }
+        });
+      } else {
+        with_activation(f.act, [&](auto act) {
+#pragma unroll
+          for (int j = 0; j < N; j += 2) {
+            const float2 o = value_of<decltype(act)::value, OutT>(make_float2(z[u][j], z[u][j + 1]));
+            z[u][j] = f.scale * o.x + x[j];
+            z[u][j + 1] = f.scale * o.y + x[j + 1];
+          }
+        });
+      }
+      store_packet<OutT>(static_cast<OutT*>(f.out) + r[u] * f.out_pitch + col[u], a.out_vec, left[u], z[u]);
+    }
   }
 }
 
@@ -598,8 +665,10 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0), lane = (int)(threadIdx.x & 31);
   const int splits = a.splits, rank = (int)blockIdx.x % splits, tile = (int)blockIdx.x / splits;
   const int S = a.stages, bn = SPLIT ? kSplitCols : a.bn;
-  constexpr uint32_t kABytes = 128u * 128u;
-  const uint32_t stage_bytes = kABytes + (uint32_t)bn * 128u, ring = base + 1024u;  // (the partial tile takes the ring's place)
+  constexpr int kParts = SPLIT ? 3 : 1;  // of an operand in a stage
+  constexpr int kStepK = step_k(SPLIT), kMmas = kStepK / 16;
+  constexpr uint32_t kABytes = 128u * kStepK * 2u, kBox = kStepK * 128u;
+  const uint32_t b_bytes = (uint32_t)(bn * kStepK) * 2u, stage_bytes = kParts * (kABytes + b_bytes), ring = base + 1024u;  // (the partial tile takes the ring's place)
   auto full_bar = [&](int s) { return base + 8u * (uint32_t)s; };
   auto empty_bar = [&](int s) { return base + 8u * (uint32_t)(kMostStages + s); };
   auto acc_full_bar = [&](int b) { return base + 8u * (uint32_t)(2 * kMostStages + b); };
@@ -628,7 +697,6 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   const int high = min(a.group_m, a.tiles_m - band * a.group_m), nt = rest / high;
   const int m0 = (band * a.group_m + rest - nt * high) * 128, n0 = nt * bn;
   const int k0 = rank * a.blocks_per_split, k1 = min(k0 + a.blocks_per_split, a.kblocks);
-  const int parts = SPLIT ? kParts : 1;
 
   if (warp == 0) {
     // ------------------------------- producer ------------------------------------------------
@@ -636,75 +704,71 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
     grid_launch_dependents();  // (the columns of tensor memory are taken)
     int s = 0;
     uint32_t ph = 0;
-    bool ok = true;
 #pragma unroll 1
-    for (int kb = k0; kb < k1 && ok; ++kb)
-#pragma unroll 1
-      for (int part = 0; part < parts; ++part) {
-        if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x2100u + (unsigned)s)) {
-          ok = false;
-          break;
-        }
-        const uint32_t fb = full_bar(s), sa = ring + (uint32_t)s * stage_bytes, sb = sa + kABytes;
-        const int ka = kb * kStepK + (SPLIT ? part_of_a(part) * a.part_k : 0), kc = kb * kStepK + (SPLIT ? part_of_b(part) * a.part_k : 0);
-        if (elect_one()) {
-          mbar_arrive_expect_tx(fb, stage_bytes);
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a, 0x2100u + (unsigned)s)) break;
+      const uint32_t fb = full_bar(s);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(fb, stage_bytes);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const uint32_t sa = ring + (uint32_t)s * stage_bytes + (uint32_t)part * kABytes;
+          const uint32_t sb = ring + (uint32_t)s * stage_bytes + kParts * kABytes + (uint32_t)part * b_bytes;
+          const int k = kb * kStepK + part * a.part_k;
           if (a.a_mn) {
-            load_2d(sa, &a.a_map, fb, m0, ka);
-            load_2d(sa + 8192u, &a.a_map, fb, m0 + 64, ka);
+            load_2d(sa, &a.a_map, fb, m0, k);
+            load_2d(sa + kBox, &a.a_map, fb, m0 + 64, k);
           } else {
-            load_2d(sa, &a.a_map, fb, ka, m0);
+            load_2d(sa, &a.a_map, fb, k, m0);
           }
           if (a.b_mn) {
-            load_2d(sb, &a.b_map, fb, n0, kc);
-            if (bn > 64) load_2d(sb + 8192u, &a.b_map, fb, n0 + 64, kc);
+            load_2d(sb, &a.b_map, fb, n0, k);
+            if (bn > 64) load_2d(sb + kBox, &a.b_map, fb, n0 + 64, k);
           } else {
-            load_2d(sb, &a.b_map, fb, kc, n0);
+            load_2d(sb, &a.b_map, fb, k, n0);
           }
         }
-        __syncwarp();
-        if (++s == S) {
-          s = 0;
-          ph ^= 1u;
-        }
       }
+      __syncwarp();
+      if (++s == S) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer -----------------------------------------------
-    const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo);
+    const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo, a.a_layout), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo, a.b_layout);
     const uint32_t a_kadv = a.a_kadv >> 4, b_kadv = a.b_kadv >> 4, idesc = a.idesc;
     int s = 0;
     uint32_t ph = 0, buf = 0, aph = 0, accumulate = 0u;
-    bool ok = true;
     grid_dependency_wait();
 #pragma unroll 1
-    for (int kb = k0; kb < k1 && ok; ++kb) {
-      if constexpr (SPLIT) {
+    for (int kb = k0; kb < k1; ++kb) {
+      const int in_chain = (kb - k0) % kChainSteps;
+      if (SPLIT && in_chain == 0) {
         if (!warp_wait(acc_empty_bar((int)buf), aph ^ 1u, abort_flag, a, 0x2200u + buf)) break;
         tc_fence_after_sync();
         accumulate = 0u;
       }
       const uint32_t d = tmem_base + (SPLIT ? buf * (uint32_t)kSplitCols : 0u);
-#pragma unroll 1
-      for (int part = 0; part < parts; ++part) {
-        if (!warp_wait(full_bar(s), ph, abort_flag, a, 0x2300u + (unsigned)s)) {
-          ok = false;
-          break;
-        }
-        const uint32_t sa = (ring + (uint32_t)s * stage_bytes) & 0x3FFFFu;
-        const uint64_t da = a_desc0 + (uint64_t)(sa >> 4), db = b_desc0 + (uint64_t)((sa + kABytes) >> 4);
-        warp_mma_f16(d, da, db, idesc, accumulate);
-        warp_mma_f16(d, da + a_kadv, db + b_kadv, idesc, 1u);
-        warp_mma_f16(d, da + 2 * a_kadv, db + 2 * b_kadv, idesc, 1u);
-        warp_mma_f16(d, da + 3 * a_kadv, db + 3 * b_kadv, idesc, 1u);
-        accumulate = 1u;
-        warp_commit(empty_bar(s));
-        if (++s == S) {
-          s = 0;
-          ph ^= 1u;
+      if (!warp_wait(full_bar(s), ph, abort_flag, a, 0x2300u + (unsigned)s)) break;
+      const uint32_t sa = (ring + (uint32_t)s * stage_bytes) & 0x3FFFFu;
+      const uint64_t da0 = a_desc0 + (uint64_t)(sa >> 4), db0 = b_desc0 + (uint64_t)((sa + kParts * kABytes) >> 4);
+#pragma unroll
+      for (int i = 0; i < (SPLIT ? kProducts : 1); ++i) {
+        const uint64_t da = da0 + (uint64_t)(part_of_a<SPLIT>(i) * (kABytes >> 4)), db = db0 + (uint64_t)((uint32_t)part_of_b<SPLIT>(i) * (b_bytes >> 4));
+#pragma unroll
+        for (uint32_t k = 0; k < kMmas; ++k) {
+          warp_mma_f16(d, da + k * a_kadv, db + k * b_kadv, idesc, accumulate);
+          accumulate = 1u;
         }
       }
-      if constexpr (SPLIT) {
-        if (!ok) break;
+      warp_commit(empty_bar(s));
+      if (++s == S) {
+        s = 0;
+        ph ^= 1u;
+      }
+      if (SPLIT && (in_chain == kChainSteps - 1 || kb + 1 == k1)) {
         warp_commit(acc_full_bar((int)buf));
         if (++buf == 2u) {
           buf = 0;
@@ -738,7 +802,7 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
       uint32_t buf = 0, aph = 0;
       bool ok = true;
 #pragma unroll 1
-      for (int kb = k0; kb < k1; ++kb) {
+      for (int kb = k0; kb < k1; kb += kChainSteps) {
         if (!warp_wait(acc_full_bar((int)buf), aph, abort_flag, a, 0x2400u + buf)) {
           ok = false;
           break;
@@ -786,40 +850,12 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   cluster_sync_all();
   // ------------------------------- the CTA's share of the result ------------------------------
   if (!*abort_flag) {
-    const Finish& f = a.f;
     grid_dependency_wait();
-    const int rows = 128 / splits, quads = a.swapped ? rows / 4 : bn / 4;  // tile rows of this CTA; fours in a line of the result
-    const int lines = a.swapped ? min(bn, f.rows - n0) : min(rows, f.rows - m0 - rank * rows);
-#pragma unroll 2
-    for (int i = (int)threadIdx.x; i < lines * quads; i += kSoloThreads) {
-      const int l = i / quads, c = (i - l * quads) * 4;
-      const long long r = a.swapped ? n0 + l : m0 + rank * rows + l;       // row and first column of the result
-      const int col = a.swapped ? m0 + rank * rows + c : n0 + c, left = f.cols - col;
-      if (left <= 0) continue;
-      const uint32_t at = base + 1024u + (a.swapped ? (uint32_t)l * line + (uint32_t)(rank * rows + c) * 4u
-                                                    : (uint32_t)(rank * rows + l) * line + (uint32_t)c * 4u);
-      float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (f.bias != nullptr) load_four<OutT>(static_cast<const OutT*>(f.bias) + col, a.bias_vec, left, v);
-      if (f.aux != nullptr) load_four<OutT>(static_cast<const OutT*>(f.aux) + r * f.aux_pitch + col, a.aux_vec, left, x);
-      float z[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < splits; ++k) {
-        const float4 p = ld_cluster_v4(cluster_map_shared(at, (uint32_t)k));
-        z[0] += p.x, z[1] += p.y, z[2] += p.z, z[3] += p.w;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += z[j];
-      if (f.pre != nullptr) store_four<OutT>(static_cast<OutT*>(f.pre) + r * f.pre_pitch + col, a.pre_vec, left, v);
-      with_activation(f.act, [&](auto act) {
-        constexpr int ACT = decltype(act)::value;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (f.gradient)
-            v[j] = f.aux != nullptr ? v[j] * slope_of<ACT, OutT>(x[j]) : v[j];
-          else
-            v[j] = f.scale * value_of<ACT, OutT>(v[j]) + x[j];
-        }
-      });
-      store_four<OutT>(static_cast<OutT*>(f.out) + r * f.out_pitch + col, a.out_vec, left, v);
+    switch (splits) {
+      case 8: finish_share<OutT, 8>(a, base + 1024u, line, m0, n0, bn, rank); break;
+      case 4: finish_share<OutT, 4>(a, base + 1024u, line, m0, n0, bn, rank); break;
+      case 2: finish_share<OutT, 2>(a, base + 1024u, line, m0, n0, bn, rank); break;
+      default: finish_share<OutT, 1>(a, base + 1024u, line, m0, n0, bn, rank);
     }
   } else {
     const uint64_t t0 = global_timer_ns();  // copies already issued may still be landing in shared memory
@@ -835,28 +871,51 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
 }
 
 // ---- fp32 operands in three parts ---------------------------------------------------------------------
-// x = p0 + p1 + p2 + (at most 2^-25 of x): each part the rest rounded to bf16, the rests themselves exact.  to[part][..]: parts are
-// `part_stride` elements apart; rows x cols of the source, zeros up to to_rows x to_cols.
-__global__ void __launch_bounds__(256) split_parts_kernel(const float* from, long long pitch, int rows, int cols, __nv_bfloat16* to,
-                                                          long long to_pitch, long long part_stride, size_t pairs, int to_cols) {
+// x = p0 + p1 + p2 + (at most 2^-25 of x): each part the rest rounded to bf16, the rests themselves exact.  Both operands in one
+// launch, eight elements of a row of the result to a thread: rows x cols of the source, zeros up to to_rows x to_cols.
+struct SplitSide {
+  const float* from;
+  __nv_bfloat16* to;
+  long long pitch, to_pitch, part_stride;
+  int rows, cols, to_cols, packets;  // packets: the source is read 16 bytes at a time
+  unsigned items, blocks;
+};
+struct SplitArgs {
+  SplitSide side[2];
+};
+__global__ void __launch_bounds__(256) split_parts_kernel(const SplitArgs a) {
   overlap_wait();
-  const int half_cols = to_cols / 2;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (size_t)gridDim.x * 256) {
-    const size_t r = i / half_cols;
-    const int c = (int)(i - r * half_cols) * 2;
-    float v[2];
+  const bool second = blockIdx.x >= a.side[0].blocks;
+  const SplitSide& s = a.side[second ? 1 : 0];
+  const unsigned step = s.blocks * 256u, pieces = (unsigned)s.to_cols / 8u;
+  for (unsigned i = (blockIdx.x - (second ? a.side[0].blocks : 0u)) * 256u + threadIdx.x; i < s.items; i += step) {
+    const unsigned r = i / pieces;
+    const int c = (int)(i - r * pieces) * 8;
+    float v[8];
+    const float* from = s.from + (long long)r * s.pitch + c;
+    if (s.packets && (int)r < s.rows && c + 8 <= s.cols) {
+      const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) v[j] = r < (size_t)rows && c + j < cols ? from[(long long)r * pitch + c + j] : 0.f;
-    __nv_bfloat162* at = reinterpret_cast<__nv_bfloat162*>(to + (long long)r * to_pitch + c);
+      for (int j = 0; j < 8; ++j) v[j] = (int)r < s.rows && c + j < s.cols ? from[j] : 0.f;
+    }
+    __nv_bfloat16* to = s.to + (long long)r * s.to_pitch + c;
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
-      __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
-      if (__hisinf(p.x)) p.x = __float2bfloat16_rz(v[0]);  // (finite values beyond bf16's largest)
-      if (__hisinf(p.y)) p.y = __float2bfloat16_rz(v[1]);
-      *at = p;
-      at += part_stride / 2;
-      v[0] -= __low2float(p);
-      v[1] -= __high2float(p);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        if (part == 0) {  // (finite values beyond bf16's largest)
+          if (__hisinf(p.x)) p.x = __float2bfloat16_rz(v[2 * j]);
+          if (__hisinf(p.y)) p.y = __float2bfloat16_rz(v[2 * j + 1]);
+        }
+        v[2 * j] -= __low2float(p);
+        v[2 * j + 1] -= __high2float(p);
+        w[j] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+      *reinterpret_cast<uint4*>(to + part * s.part_stride) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -879,8 +938,9 @@ EncodeFn encoder() {
   return fn;
 }
 
-// Boxes of 128 bytes x box_rows of a matrix of rows x cols elements, zeros outside it, swizzled.
-bool matrix_map(CUtensorMap* map, int dtype, const void* p, long long pitch, long long rows, long long cols, int box_rows) {
+// Boxes of row_bytes (128 or 64) x box_rows of a matrix of rows x cols elements, zeros outside it, swizzled.
+bool matrix_map(CUtensorMap* map, int dtype, const void* p, long long pitch, long long rows, long long cols, int box_rows,
+                int row_bytes = 128) {
   const EncodeFn fn = encoder();
   if (fn == nullptr) {
     fail(PDNN_ALLOCATION_PROBLEM, "cuTensorMapEncodeTiled is unavailable");
@@ -889,12 +949,12 @@ bool matrix_map(CUtensorMap* map, int dtype, const void* p, long long pitch, lon
   const cuuint64_t es = dtype_size(dtype);
   if (rows == 1) pitch = (long long)((cols * es + 15) / 16 * 16 / es);  // (no row follows)
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * es};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)(row_bytes / es), (cuuint32_t)box_rows}, ones[2] = {1, 1};
   const CUtensorMapDataType dt = dtype == PDNN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                : dtype == PDNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUresult r = fn(map, dt, 2, const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     fail(PDNN_INVALID_PARAMETER, "cuTensorMapEncodeTiled failed (%d): %lld x %lld, pitch %lld", (int)r, rows, cols, pitch);
   return r == CUDA_SUCCESS;
@@ -904,8 +964,8 @@ bool tma_ok(int dtype, const void* p, long long pitch, int rows) {
   const long long bytes = pitch * (long long)dtype_size(dtype);
   return aligned16(p) && (rows == 1 || (bytes % 16 == 0 && bytes < (1ll << 40)));
 }
-bool fours_ok(int dtype, const void* p, long long pitch) {
-  return reinterpret_cast<uintptr_t>(p) % (4 * dtype_size(dtype)) == 0 && pitch % 4 == 0;
+bool packets_ok(int dtype, const void* p, long long pitch) {
+  return aligned16(p) && pitch * (long long)dtype_size(dtype) % 16 == 0;
 }
 
 // An operand as the kernels see it: `mn` rows or columns of the tile's side, MN-major or K-major.
@@ -915,27 +975,28 @@ struct Side {
   int mn, mn_major;
 };
 
-constexpr int kPairStage256 = 32768, kPairStage128 = 24576;
-
 struct Plan {
   bool pair;
   int bn, splits;
   bool swapped;
 };
 
-// Estimated time in cycles of the plans, from what bounds them: an SM takes a 128 x 256 x 64 step of a pair's tile in 512 cycles; a CTA
-// alone pulls its operands of 16 KB + 128 B a column through L2 at about 40 bytes a cycle while all SMs do, and a step takes
-// it no less than 150 cycles.  A pair's tile ends with about 2500 cycles (the last one's end is not hidden), a CTA's with
-// 2500 and 400 for each partial tile it adds.
+// Estimated times of the plans in us, from what they measured over 24 shapes of 1 to 8192 rows (a step is 64 elements of K).
+// A pair's step takes 0.34 us at 256 columns and 0.23 at 128 (an SM pulls its 24 KB of operands through L2 no faster), two
+// thirds of that with few clusters in flight, behind 5.5 and 4.7 us of launch, ramp and end.  A CTA alone takes 0.2 to 0.29 us a step
+// by its columns, half as much again where two share an SM, behind 3 us, 0.017 a column for its end and 0.45 for each
+// partial tile that it adds.
 Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_major, int kblocks, int sms) {
-  const double parts = split ? kParts : 1;
+  const double products = split ? kProducts : 1;
   auto tiles = [](long long x, int t) { return (x + t - 1) / t; };
   Plan best{true, 128, 1, false};
   double least = 1e30;
   for (int bn : {256, 128}) {
     if (split && bn == 256) continue;
-    const double waves = (double)tiles(tiles(m, 256) * tiles(n, bn), sms / 2);
-    const double t = waves * kblocks * parts * 2.0 * bn + 3500 + (split ? 2000 : 0);
+    const long long all = tiles(m, 256) * tiles(n, bn);
+    const double waves = (double)tiles(all, sms / 2), busy = std::min(1.0, (double)all / (sms / 2));
+    const double step = (bn == 256 ? 0.34 : 0.23) * (0.6 + 0.4 * busy);
+    const double t = waves * kblocks * step * products + (bn == 256 ? 5.5 : 4.7) + (split ? 2.0 : 0.0);
     if (t < least) least = t, best = Plan{true, bn, 1, false};
   }
   for (int swapped = 0; swapped < 2; ++swapped)
@@ -943,15 +1004,15 @@ Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_majo
       if (split && bn != kSplitCols) continue;
       if (bn < 64 && (swapped ? m_major : n_major)) continue;  // (an MN-major tile is whole boxes of 64 columns)
       const long long rows = swapped ? n : m, cols = swapped ? m : n;
-      const long long t1 = tiles(rows, 128) * tiles(cols, bn);
-      if (t1 > 8ll * sms) continue;
+      const long long all = tiles(rows, 128) * tiles(cols, bn);
+      if (all > 8ll * sms) continue;
       for (int splits : {1, 2, 4, 8}) {
-        if (splits > 1 && (kblocks + splits - 1) / splits * (splits - 1) >= kblocks) continue;  // a CTA without steps
-        const long long ctas = t1 * splits;
-        const double steps = (double)((kblocks + splits - 1) / splits) * parts;
-        const double step = std::max(150.0, (16384.0 + 128.0 * bn) / 40.0);
-        const double waves = (double)tiles(ctas, sms);
-        const double t = waves * steps * step + (ctas > 2 * sms ? waves / 2 : 1) * (2500 + 400 * splits);
+        const int steps = (kblocks + splits - 1) / splits;
+        if (splits > 1 && steps * (splits - 1) >= kblocks) continue;  // a CTA without steps
+        const long long ctas = all * splits;
+        const double waves = (double)tiles(ctas, 2ll * sms), shared = ctas > sms ? 1.5 : 1.0;
+        const double step = (bn == 128 ? 0.29 : bn == 64 ? 0.23 : 0.2) * shared;
+        const double t = 1.5 + waves * (steps * step * products + 1.5 + 0.017 * bn * shared + (splits > 1 ? 0.45 * splits : 0.0));
         if (t < least) least = t, best = Plan{false, bn, splits, swapped != 0};
       }
     }
@@ -1013,27 +1074,39 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
   if (plan.swapped) std::swap(x, y);
   const int bm = plan.pair ? 256 : 128;
   a.f = f;
+  if (f.gradient && f.aux == nullptr) {  // the product alone
+    a.f.gradient = 0;
+    a.f.act = PDNN_ACT_NONE;
+  }
   a.error_record = tc_error_record_address();
   if (a.error_record == nullptr) return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: no error record");
   a.wait_limit_ns = kWaitLimitNs;
   a.tiles_m = (x.mn + bm - 1) / bm;
   a.tiles_n = (y.mn + plan.bn - 1) / plan.bn;
   a.group_m = std::min(a.tiles_m, 8);
+  constexpr int kStepK = step_k(SPLIT);
   a.kblocks = (k + kStepK - 1) / kStepK;
   a.part_k = part_k;
   a.a_mn = x.mn_major;
   a.b_mn = y.mn_major;
-  a.a_lbo = x.mn_major ? 8192u : 16u;
-  a.b_lbo = y.mn_major ? 8192u : 16u;
-  a.a_sbo = a.b_sbo = 1024u;
+  // MN-major: k-rows of 128 bytes, 64 columns after 64 columns; K-major: rows of one step, 128 bytes or 64, swizzled accordingly
+  const unsigned row = kStepK * 2u;
+  a.a_lbo = x.mn_major ? kStepK * 128u : 16u;
+  a.b_lbo = y.mn_major ? kStepK * 128u : 16u;
+  a.a_sbo = x.mn_major ? 1024u : 8u * row;
+  a.b_sbo = y.mn_major ? 1024u : 8u * row;
+  a.a_layout = x.mn_major || row == 128u ? 2u : 4u;
+  a.b_layout = y.mn_major || row == 128u ? 2u : 4u;
   a.a_kadv = x.mn_major ? 2048u : 32u;
   a.b_kadv = y.mn_major ? 2048u : 32u;
   a.idesc = make_idesc(dtype == PDNN_BF16 ? 1 : 0, x.mn_major, y.mn_major, plan.bn, plan.pair ? 256 : 128);
   const long long depth = SPLIT ? 3ll * part_k : k;  // elements along K in memory
   const int b_cols = plan.pair ? plan.bn / 2 : plan.bn;
-  if (!matrix_map(&a.a_map, dtype, x.p, x.pitch, x.mn_major ? depth : x.mn, x.mn_major ? x.mn : depth, x.mn_major ? kStepK : 128) ||
-      !matrix_map(&a.b_map, dtype, y.p, y.pitch, y.mn_major ? depth : y.mn, y.mn_major ? y.mn : depth, y.mn_major ? kStepK : b_cols))
-    return PDNN_INVALID_PARAMETER;
+  auto operand_map = [&](CUtensorMap* map, const Side& side, int cols) {
+    return side.mn_major ? matrix_map(map, dtype, side.p, side.pitch, depth, side.mn, kStepK)
+                         : matrix_map(map, dtype, side.p, side.pitch, side.mn, depth, cols, (int)row);
+  };
+  if (!operand_map(&a.a_map, x, 128) || !operand_map(&a.b_map, y, b_cols)) return PDNN_INVALID_PARAMETER;
   if (plan.pair) {
     a.out_tma = tma_ok(out_dtype, f.out, f.out_pitch, f.rows);
     a.aux_tma = f.aux != nullptr && tma_ok(out_dtype, f.aux, f.aux_pitch, f.rows);
@@ -1042,7 +1115,7 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
         (a.aux_tma && !matrix_map(&a.aux_map, out_dtype, f.aux, f.aux_pitch, f.rows, f.cols, 32)) ||
         (a.pre_tma && !matrix_map(&a.pre_map, out_dtype, f.pre, f.pre_pitch, f.rows, f.cols, 32)))
       return PDNN_INVALID_PARAMETER;
-    const int stage = plan.bn == 256 ? kPairStage256 : kPairStage128;
+    const int stage = (SPLIT ? 3 : 1) * (128 + plan.bn / 2) * kStepK * 2;
     const int fixed = 1024 + 2 * kEndWarps * kSlotBytes + 8 * (2 * kMostStages + 4 + 2 * kEndWarps) + 16 + kEndWarps * 128;
     a.stages = std::min(kMostStages, (kSmemBudget - fixed) / stage);
     const unsigned grid = (unsigned)std::min<long long>(2ll * a.tiles_m * a.tiles_n, sms / 2 * 2);
@@ -1056,15 +1129,15 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
   }
   a.bn = plan.bn;
   a.splits = plan.splits;
-  a.blocks_per_split = (a.kblocks + plan.splits - 1) / plan.splits;
+  a.blocks_per_split = ((k + 63) / 64 + plan.splits - 1) / plan.splits * (64 / kStepK);
   a.swapped = plan.swapped;
   const int columns = SPLIT ? 2 * kSplitCols : plan.bn;
   a.tmem_cols = std::max(32, columns);
-  a.out_vec = fours_ok(out_dtype, f.out, f.out_pitch);
-  a.aux_vec = fours_ok(out_dtype, f.aux, f.aux_pitch);
-  a.pre_vec = fours_ok(out_dtype, f.pre, f.pre_pitch);
-  a.bias_vec = fours_ok(out_dtype, f.bias, 0);
-  const int stage = 16384 + plan.bn * 128;
+  a.out_vec = packets_ok(out_dtype, f.out, f.out_pitch);
+  a.aux_vec = packets_ok(out_dtype, f.aux, f.aux_pitch);
+  a.pre_vec = packets_ok(out_dtype, f.pre, f.pre_pitch);
+  a.bias_vec = packets_ok(out_dtype, f.bias, 0);
+  const int stage = (SPLIT ? 3 : 1) * (128 + plan.bn) * kStepK * 2;
   a.stages = std::min(kMostStages, (kSoloSmem - kSoloHead) / stage);
   const size_t partial = plan.swapped ? (size_t)plan.bn * (128 * 4 + 16) : (size_t)128 * (plan.bn * 4 + 16);
   const size_t smem = kSoloHead + std::max((size_t)a.stages * stage, partial);
@@ -1080,12 +1153,15 @@ bool fused_gemm_operand_ok(int dtype, const Matrix& m) { return dtype == PDNN_F3
 int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, cudaStream_t s) {
   const int sms = device_sm_count();
   Side x{a.p, a.pitch, f.rows, ta}, y{b.p, b.pitch, f.cols, !tb};
-  const int kblocks = (k + kStepK - 1) / kStepK;
+  const int kblocks = (k + 63) / 64;
   Plan plan = choose_plan(dtype == PDNN_F32, f.rows, f.cols, x.mn_major != 0, y.mn_major != 0, kblocks, sms);
   if (dtype == PDNN_F16) return run_plan<__half, false>(plan, dtype, dtype, x, y, k, 0, f, s);
   if (dtype == PDNN_BF16) return run_plan<__nv_bfloat16, false>(plan, dtype, dtype, x, y, k, 0, f, s);
+  // fp32.  Few rows: cutting the weights into parts costs more than multiplying them (4096 x 4096, us, parts / rows: 1 row 59 / 15, 16
+  // rows 59 / 47, 32 rows 60 / 78).
+  if (!ta && f.rows <= kFewRows) return fused_rows(tb != 0, a, b, k, f, s);
   // parts behind one another along K
-  const int part_k = kblocks * kStepK;
+  const int part_k = kblocks * 64;
   const Matrix* from[2] = {&a, &b};
   Side* side[2] = {&x, &y};
   size_t bytes[2], cols[2];
@@ -1099,19 +1175,30 @@ int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int 
     cudaGetLastError();
     return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: cannot allocate %zu bytes of scratch", bytes[0] + bytes[1]);
   }
-  int st = PDNN_OK;
-  for (int i = 0; i < 2 && st == PDNN_OK; ++i) {
-    __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(scratch + (i == 0 ? 0 : bytes[0]));
-    const size_t rows = side[i]->mn_major ? (size_t)part_k : (size_t)side[i]->mn;
-    const long long pitch = side[i]->mn_major ? (long long)cols[i] : 3ll * part_k;
-    const long long part_stride = side[i]->mn_major ? (long long)part_k * (long long)cols[i] : part_k;
-    const size_t pairs = rows * (cols[i] / 2);
-    launch_overlapped(split_parts_kernel, grid_for(pairs, 256, sms), 256, s, static_cast<const float*>(from[i]->p), from[i]->pitch,
-                      from[i]->rows, from[i]->cols, to, pitch, part_stride, pairs, (int)cols[i]);
-    st = check_launch("matmul_fused: parts");
-    side[i]->p = to;
-    side[i]->pitch = pitch;
+  SplitArgs split;
+  for (int i = 0; i < 2; ++i) {
+    SplitSide& q = split.side[i];
+    const size_t rows = side[i]->mn_major ? (size_t)part_k : (size_t)side[i]->mn, items = rows * (cols[i] / 8);
+    if (items > 0x80000000u) {
+      cudaFreeAsync(scratch, s);
+      return fail(PDNN_INDEX_EXCEEDED, "matmul_fused: an fp32 operand of more than 2^34 elements");
+    }
+    q.from = static_cast<const float*>(from[i]->p);
+    q.to = reinterpret_cast<__nv_bfloat16*>(scratch + (i == 0 ? 0 : bytes[0]));
+    q.pitch = from[i]->pitch;
+    q.to_pitch = side[i]->mn_major ? (long long)cols[i] : 3ll * part_k;
+    q.part_stride = side[i]->mn_major ? (long long)part_k * (long long)cols[i] : part_k;
+    q.rows = from[i]->rows;
+    q.cols = from[i]->cols;
+    q.to_cols = (int)cols[i];
+    q.packets = packets_ok(PDNN_F32, from[i]->p, from[i]->pitch);
+    q.items = (unsigned)items;
+    q.blocks = grid_for(items, 256, sms);
+    side[i]->p = q.to;
+    side[i]->pitch = q.to_pitch;
   }
+  launch_overlapped(split_parts_kernel, split.side[0].blocks + split.side[1].blocks, 256, s, split);
+  int st = check_launch("matmul_fused: parts");
   if (st == PDNN_OK) st = run_plan<float, true>(plan, PDNN_BF16, PDNN_F32, x, y, k, part_k, f, s);
   cudaFreeAsync(scratch, s);
   return st;

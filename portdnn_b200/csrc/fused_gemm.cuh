@@ -13,7 +13,7 @@ struct Matrix {
 };
 
 // What is made of a product: forward  pre = v + bias, out = aux + scale * act(v + bias);
-// gradient  out = v * act'(aux).  Null tensors are left out.  rows x cols elements, pitches in elements.
+// gradient  out = scale * v * act'(aux).  Null tensors are left out.  rows x cols elements, pitches in elements.
 struct Finish {
   const void* bias;
   const void* aux;
@@ -29,5 +29,8 @@ struct Finish {
 // alignment are cut into three bf16 parts in scratch.
 bool fused_gemm_operand_ok(int dtype, const Matrix& m);
 int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, cudaStream_t s);
+
+// The same for a few fp32 rows x (row-major) and weights w, stored [f.cols][k] (k_rows) or [k][f.cols] (fused_rows.cu).
+int fused_rows(bool k_rows, const Matrix& x, const Matrix& w, int k, const Finish& f, cudaStream_t s);
 
 }  // namespace pdnn

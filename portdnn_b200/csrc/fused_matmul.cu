@@ -105,30 +105,39 @@ __global__ void __launch_bounds__(32 * kSlopeLanes) activation_slope_kernel(cons
   const int col = ((int)blockIdx.x * 32 + tx) * V;
   const int first = (int)blockIdx.y * a.rows_per_slice, last = min(first + a.rows_per_slice, a.m);
   float sum[V] = {};
-  if (col < a.n) {
-#pragma unroll 2
-    for (int r = first + ty; r < last; r += kSlopeLanes) {
-      const T* dy = static_cast<const T*>(a.dy) + (long long)r * a.dy_pitch + col;
-      const T* pre = static_cast<const T*>(a.pre) + (long long)r * a.pre_pitch + col;
-      float v[V];
-      if constexpr (V == 1) {
-        v[0] = a.scale * to_f32(*dy) * (a.pre != nullptr ? activation_slope(a.act, to_f32(*pre)) : 1.f);
-        if (a.dz != nullptr) static_cast<T*>(a.dz)[(long long)r * a.dz_pitch + col] = from_f32<T>(v[0]);
-      } else {
-        const Vec16<T> d = load16(dy);
-        Vec16<T> z = d, o;
-        if (a.pre != nullptr) z = load16(pre);
+  if (col < a.n)
+    with_activation(a.pre != nullptr ? a.act : PDNN_ACT_NONE, [&](auto act) {
+      constexpr int ACT = decltype(act)::value, kAhead = V == 1 ? 8 : 4;  // rows of a thread whose loads are in flight together
+      for (int r0 = first + ty; r0 < last; r0 += kAhead * kSlopeLanes) {
+        Piece<T, V> d[kAhead], z[kAhead];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          v[i] = a.scale * to_f32(d.get(i)) * (a.pre != nullptr ? activation_slope(a.act, to_f32(z.get(i))) : 1.f);
-          o.set(i, from_f32<T>(v[i]));
+        for (int u = 0; u < kAhead; ++u) {
+          const int r = r0 + u * kSlopeLanes;
+          if (r >= last) continue;
+          d[u].load(static_cast<const T*>(a.dy) + (long long)r * a.dy_pitch + col);
+          if (ACT != PDNN_ACT_NONE) z[u].load(static_cast<const T*>(a.pre) + (long long)r * a.pre_pitch + col);
         }
-        if (a.dz != nullptr) store16(static_cast<T*>(a.dz) + (long long)r * a.dz_pitch + col, o);
-      }
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += v[i];
-    }
-  }
+        for (int u = 0; u < kAhead; ++u) {
+          const int r = r0 + u * kSlopeLanes;
+          if (r >= last) continue;
+          Piece<T, V> o;
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            constexpr int kNext = V > 1 ? 1 : 0;
+            float2 v = make_float2(a.scale * d[u].get(i), a.scale * d[u].get(i + kNext));
+            if (ACT != PDNN_ACT_NONE) v = mul2(v, slope_of<ACT, T>(make_float2(z[u].get(i), z[u].get(i + kNext))));
+            o.set(i, v.x);
+            sum[i] += v.x;
+            if (V > 1) {
+              o.set(i + kNext, v.y);
+              sum[i + kNext] += v.y;
+            }
+          }
+          if (a.dz != nullptr) o.store(static_cast<T*>(a.dz) + (long long)r * a.dz_pitch + col);
+        }
+      }
+    });
   if (a.partial == nullptr) return;
 #pragma unroll
   for (int i = 0; i < V; ++i) red[ty][tx * V + i] = sum[i];
@@ -218,7 +227,9 @@ int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, c
     return PDNN_OK;
   }
   Matrix dz{grad, p.output_pitch, p.m, p.n};
-  const bool own = (g.activation != PDNN_ACT_NONE || g.scale != 1.f) && (g.lhs_grad != nullptr || g.rhs_grad != nullptr);
+  // (without an activation dz is dy, and the scale goes into the products' ends)
+  const bool own = g.activation != PDNN_ACT_NONE && (g.lhs_grad != nullptr || g.rhs_grad != nullptr);
+  const float end_scale = g.activation != PDNN_ACT_NONE ? 1.f : g.scale;
   Scratch scratch(s);
   if (own || g.bias_grad != nullptr) {
     const long long pitch = (long long)round_up(p.n, 16 / es);
@@ -238,6 +249,7 @@ int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, c
     f.rows = p.m;
     f.cols = p.k;
     f.act = g.input_activation;
+    f.scale = end_scale;
     f.gradient = 1;
     f.aux = g.input_activation != PDNN_ACT_NONE ? g.input_pre_activation : nullptr;
     f.aux_pitch = g.input_pre_activation_pitch;
@@ -251,6 +263,7 @@ int launch_matmul_fused_gradient(int dtype, const void* grad, const void* lhs, c
     f.rows = w_rows;
     f.cols = w_cols;
     f.act = PDNN_ACT_NONE;
+    f.scale = end_scale;
     f.gradient = 1;
     const Matrix x{lhs, p.lhs_pitch, p.m, p.k};
     const int st = p.transpose_rhs ? product(dtype, 1, 0, dz, x, p.m, f, s) : product(dtype, 1, 0, x, dz, p.m, f, s);

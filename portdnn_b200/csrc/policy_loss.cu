@@ -17,11 +17,12 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace pdnn {
 namespace {
 
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;  // (log2 e, ln 2)
 
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
@@ -39,15 +40,15 @@ struct LossArgs {
   float c, inv_temperature, clip_low, clip_high, kl, grad_scale;  // c = log2(e) / temperature
 };
 
-// The largest value so far and the sum of 2^((v - top) * c).  Of values that are all minus infinity the sum is 0.
+// Sums of 2^(x c - shift): the shift is the largest x so far times c, rounded, and cancels from every result, so that its
+// rounding does no harm.  Of values that are all minus infinity the sum is 0 and the shift minus infinity.
 struct alignas(8) Partial {
-  float top, sum;
+  float shift, sum;
 };
-__device__ __forceinline__ Partial merge(Partial a, Partial b, float c) {
-  const float top = fmaxf(a.top, b.top);
-  // (equal tops, infinite ones among them, need no scaling; NaN sums stay NaN)
-  const float fa = a.top == top ? 1.f : exp2_fast((a.top - top) * c), fb = b.top == top ? 1.f : exp2_fast((b.top - top) * c);
-  return Partial{top, a.sum * fa + b.sum * fb};
+__device__ __forceinline__ float scale_to(float from, float to) { return from == to ? 1.f : exp2_fast(from - to); }  // (both may be infinite)
+__device__ __forceinline__ Partial merge(Partial a, Partial b) {
+  const float shift = fmaxf(a.shift, b.shift);
+  return Partial{shift, a.sum * scale_to(a.shift, shift) + b.sum * scale_to(b.shift, shift)};
 }
 
 template <typename T>
@@ -55,7 +56,21 @@ __device__ __forceinline__ void store_streaming(T* p, const Vec16<T>& v) {
   __stcs(reinterpret_cast<uint4*>(p), v.raw);
 }
 
-// One row to a cluster of CTAs (most often to a CTA).
+// Two neighbouring results as one word, rounded.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_word(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// One row to a cluster of CTAs (most often to a CTA).  An element costs an exponential in either walk, and as little else as
+// possible: product and shift are one multiply-add, the gradient's factor is added to the exponent and its sign put
+// on afterwards, and the chosen token's entry is written over at the end.
 template <typename T>
 __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
   overlap_wait();
@@ -96,20 +111,27 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
   const float chosen = tid == 0 ? to_f32(x[t]) : 0.f;
   Partial part{-INFINITY, 0.f};
   auto take = [&](const float* v, int n) {
-    float top = part.top;
-    for (int i = 0; i < n; ++i) top = fmaxf(top, v[i]);
-    if (top > part.top) {
-      part.sum *= exp2_fast((part.top - top) * a.c);  // (from minus infinity: 0 times 0)
-      part.top = top;
+    float top = v[0];
+    for (int i = 1; i < n; ++i) top = fmaxf(top, v[i]);
+    const float shift = top * a.c;
+    if (shift > part.shift) {
+      part.sum *= exp2_fast(part.shift - shift);  // (from minus infinity: 0 times 0)
+      part.shift = shift;
     }
-    if (part.top == -INFINITY) {  // nothing but minus infinity, or NaN, which fmaxf passes over
+    if (part.shift == -INFINITY) {  // nothing but minus infinity, or NaN, which fmaxf passes over
       for (int i = 0; i < n; ++i)
         if (v[i] != v[i]) part.sum = v[i];
       return;
     }
     float sum = 0.f;
-    for (int i = 0; i < n; ++i) sum += exp2_fast((v[i] - part.top) * a.c);
+    for (int i = 0; i < n; ++i) sum += exp2_fast(fmaf(v[i], a.c, -part.shift));
     part.sum += sum;
+  };
+  auto take_packet = [&](const Vec16<T>& p) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(p.get(i));
+    take(v, N);
   };
   {
     int j = begin + tid * N;
@@ -118,20 +140,9 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * threads * N);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        float v[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_f32(p[u].get(i));
-        take(v, N);
-      }
+      for (int u = 0; u < kUnroll; ++u) take_packet(p[u]);
     }
-    for (; j < packed_end; j += threads * N) {
-      const Vec16<T> p = load16(x + j);
-      float v[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = to_f32(p.get(i));
-      take(v, N);
-    }
+    for (; j < packed_end; j += threads * N) take_packet(load16(x + j));
     for (int k = packed_end + tid; k < end; k += threads) {
       const float v = to_f32(x[k]);
       take(&v, 1);
@@ -139,29 +150,31 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const Partial other{__shfl_xor_sync(0xFFFFFFFFu, part.top, o), __shfl_xor_sync(0xFFFFFFFFu, part.sum, o)};
-    part = merge(part, other, a.c);
+    const Partial other{__shfl_xor_sync(0xFFFFFFFFu, part.shift, o), __shfl_xor_sync(0xFFFFFFFFu, part.sum, o)};
+    part = merge(part, other);
   }
   if ((tid & 31) == 0) warp_part[tid >> 5] = part;
   __syncthreads();
   part = warp_part[0];
-  for (int w = 1; w < threads / 32; ++w) part = merge(part, warp_part[w], a.c);
+  for (int w = 1; w < threads / 32; ++w) part = merge(part, warp_part[w]);
   if (ranks > 1) {
     if (tid == 0) cta_part = part;
+    __syncwarp();
     umma::cluster_sync_all();
     const uint32_t mine = umma::smem_u32(&cta_part);
     for (uint32_t r = 0; r < ranks; ++r) {
       Partial other;
       const uint32_t at = umma::cluster_map_shared(mine, r);
-      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(other.top), "=f"(other.sum) : "r"(at) : "memory");
-      part = r == 0 ? other : merge(part, other, a.c);
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(other.shift), "=f"(other.sum) : "r"(at) : "memory");
+      part = r == 0 ? other : merge(part, other);
     }
     umma::cluster_sync_all();  // nobody leaves while its sums are read
   }
+  float chosen_grad = 0.f;
   if (tid == 0) {
     float slope = 0.f, loss = 0.f, lp = 0.f;
-    if (!(part.top == -INFINITY && part.sum == 0.f)) {  // (a row of nothing but minus infinity counts for nothing)
-      lp = (chosen - part.top) * a.inv_temperature - log2f(part.sum) * kLn2;
+    if (!(part.shift == -INFINITY && part.sum == 0.f)) {  // (a row of nothing but minus infinity counts for nothing)
+      lp = (fmaf(chosen, a.c, -part.shift) - log2f(part.sum)) * kLn2;
       const float adv = a.advantages[row];
       const float ratio = a.old_logp != nullptr ? expf(lp - a.old_logp[row]) : 1.f;
       const float open = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * adv;
@@ -175,6 +188,7 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
       }
       loss *= weight;
       slope *= weight * a.grad_scale * a.inv_temperature;
+      chosen_grad = slope - slope * (exp2_fast(fmaf(chosen, a.c, -part.shift)) / part.sum);
     }
     shared_slope = slope;
     if (rank == 0) {
@@ -184,33 +198,50 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
   }
   if (g == nullptr) return;
   __syncthreads();
-  const float slope = shared_slope, top = part.top == -INFINITY ? 0.f : part.top;
-  const float k = part.sum == 0.f ? 0.f : -slope / part.sum;
-  const int target = (int)t;
-  auto gradient = [&](float v, int j) { return exp2_fast((v - top) * a.c) * k + (j == target ? slope : 0.f); };
-  {
-    int j = begin + tid * N;
-    for (; j + (kUnroll - 1) * threads * N < packed_end; j += kUnroll * threads * N) {
-      Vec16<T> p[kUnroll];
+  // -slope * p_j = -sign(slope) * 2^(x_j c - shift + log2(|slope| / sum)), but for a slope of 0 (NaN stays NaN)
+  const float slope = shared_slope;
+  const float lift = log2f(fabsf(slope) / part.sum) - part.shift;
+  const bool none = slope == 0.f;
+  const uint32_t sign = slope > 0.f ? 0x80008000u : 0u;
+  auto packet = [&](const Vec16<T>& p) {
+    Vec16<T> o;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t w[4];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * threads * N);
+      for (int i = 0; i < 4; ++i) w[i] = pair_word<T>(exp2_fast(fmaf(to_f32(p.get(2 * i)), a.c, lift)), exp2_fast(fmaf(to_f32(p.get(2 * i + 1)), a.c, lift))) ^ sign;
+      o.raw = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        Vec16<T> o;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o.set(i, from_f32<T>(gradient(to_f32(p[u].get(i)), j + u * threads * N + i)));
-        store_streaming(g + j + u * threads * N, o);
+      for (int i = 0; i < N; ++i) {
+        const float e = exp2_fast(fmaf(to_f32(p.get(i)), a.c, lift));
+        o.set(i, from_f32<T>(slope > 0.f ? -e : e));
       }
     }
-    for (; j < packed_end; j += threads * N) {
-      const Vec16<T> p = load16(x + j);
-      Vec16<T> o;
+    return o;
+  };
+  const int kStep = threads * N;
+  if (none) {
+    Vec16<T> zero;
+    zero.raw = make_uint4(0u, 0u, 0u, 0u);
+    for (int j = begin + tid * N; j < packed_end; j += kStep) store_streaming(g + j, zero);
+    for (int j = packed_end + tid; j < end; j += threads) g[j] = from_f32<T>(0.f);
+  } else {
+    int j = begin + tid * N;
+    for (; j + (kUnroll - 1) * kStep < packed_end; j += kUnroll * kStep) {
+      Vec16<T> p[kUnroll];
 #pragma unroll
-      for (int i = 0; i < N; ++i) o.set(i, from_f32<T>(gradient(to_f32(p.get(i)), j + i)));
-      store_streaming(g + j, o);
+      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * kStep);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) store_streaming(g + j + u * kStep, packet(p[u]));
     }
-    for (int j1 = packed_end + tid; j1 < end; j1 += threads) g[j1] = from_f32<T>(gradient(to_f32(x[j1]), j1));
+    for (; j < packed_end; j += kStep) store_streaming(g + j, packet(load16(x + j)));
+    for (int j1 = packed_end + tid; j1 < end; j1 += threads) {
+      const float e = exp2_fast(fmaf(to_f32(x[j1]), a.c, lift));
+      g[j1] = from_f32<T>(slope > 0.f ? -e : e);
+    }
   }
+  __syncthreads();
+  if (tid == 0 && t >= begin && t < end) g[t] = from_f32<T>(chosen_grad);
 }
 
 // The sum of the tokens' losses, in one order.

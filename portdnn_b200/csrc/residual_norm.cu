@@ -11,8 +11,10 @@
 // Bound by memory: forward reads two tensors and writes two, backward reads four and writes two, each once.  A
 // team of threads keeps a row in registers (a packet or two to a thread), so that statistics over the row - taken
 // about the mean, in fp32 - cost no second read, and requests the next row before it reduces this one.  Teams keep to
-// whole stretches of rows: gamma, beta and the gate stay in registers, and the sums over rows of the backward pass are
-// the thread's own until its stretch ends.  They end in one line of partial sums a team, which column_sums.cuh
+// whole stretches of rows: what depends on the column alone stays in registers, multiplied out (scale * act(gate) * gamma
+// is one number), and the sums over rows of the backward pass are the thread's own until its stretch ends.  Both of
+// the gradients behind the post norm's result come of one sum over the group's rows, P = sum ds * hat: gamma's is
+// scale * act(gate) * P, the gate's scale * act'(gate) * gamma * P.  A team leaves one line of partial sums, which column_sums.cuh
 // adds in a fixed order.
 #include "activation.cuh"
 #include "column_sums.cuh"
@@ -20,27 +22,10 @@
 #include <algorithm>
 #include <cstring>
 #include <initializer_list>
+#include <type_traits>
 
 namespace pdnn {
 namespace {
-
-// V elements as a thread keeps them: a 16-byte packet or a single element.
-template <typename T, int V>
-struct Piece {
-  Vec16<T> raw;
-  __device__ __forceinline__ void load(const T* p) { raw = load16(p); }
-  __device__ __forceinline__ float get(int i) const { return to_f32(raw.get(i)); }
-  __device__ __forceinline__ void set(int i, float v) { raw.set(i, from_f32<T>(v)); }
-  __device__ __forceinline__ void store(T* p) const { store16(p, raw); }
-};
-template <typename T>
-struct Piece<T, 1> {
-  T raw;
-  __device__ __forceinline__ void load(const T* p) { raw = *p; }
-  __device__ __forceinline__ float get(int) const { return to_f32(raw); }
-  __device__ __forceinline__ void set(int, float v) { raw = from_f32<T>(v); }
-  __device__ __forceinline__ void store(T* p) const { *p = raw; }
-};
 
 struct NormArgs {
   const void *branch, *residual, *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
@@ -51,8 +36,12 @@ struct NormArgs {
   // backward
   const void *sum_grad, *out_grad;
   void *branch_grad, *residual_grad, *gate_grad;
-  float *partial, *gate_partial;  // [teams][vectors][channels], [parts][groups][channels]
-  int parts, vectors;             // stretches of rows that a group is cut into; parameter vectors with a gradient
+  // Partial sums: a line of `line` floats to a team, the parameter vectors' behind one another; to each part of the groups
+  // gate_line floats from gate_partial on, [groups][channels] (with one group a further vector of the same lines).
+  float *partial, *gate_partial;
+  size_t line, gate_line;
+  int parts;    // stretches of rows that a group is cut into
+  int vectors;  // parameter vectors with a gradient
   int slot[4];                    // where in a line of `partial` post gamma, post beta, pre gamma, pre beta are; -1: nowhere
 };
 
@@ -89,13 +78,13 @@ struct TeamSum {
 constexpr int block_of(int team) { return team == 32 ? 256 : team; }
 
 // Mean and r of a row that a team holds; entries behind the row's end are zero and `live` says which are not.
-template <int V, int NP, typename Sum>
+template <int V, int NP, bool LAYER, typename Sum>
 __device__ __forceinline__ void row_statistics(int kind, const float (&v)[NP][V], const bool (&live)[NP], float inv_channels,
                                                float epsilon, Sum& team_sum, float& mean, float& r) {
   mean = 0.f;
   r = 1.f;
   if (kind == PDNN_NORM_NONE) return;
-  if (kind == PDNN_NORM_LAYER) {
+  if (LAYER && kind == PDNN_NORM_LAYER) {
     float total = 0.f;
 #pragma unroll
     for (int p = 0; p < NP; ++p)
@@ -108,28 +97,20 @@ __device__ __forceinline__ void row_statistics(int kind, const float (&v)[NP][V]
   for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float d = v[p][i] - mean;
-      if (live[p]) squares += d * d;
+      const float d = LAYER ? v[p][i] - mean : v[p][i];
+      if (!LAYER || live[p]) squares += d * d;  // (entries that are not live are zero)
     }
   r = 1.f / sqrtf(team_sum(squares, 0.f).x * inv_channels + epsilon);
 }
 
-template <typename T, int V, int NP>
-__device__ __forceinline__ void load_vector(const void* from, float fill, const bool (&live)[NP], const int (&at)[NP],
-                                            Piece<T, V> (&to)[NP]) {
-#pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    if (from != nullptr && live[p]) {
-      to[p].load(static_cast<const T*>(from) + at[p]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) to[p].set(i, fill);
-    }
-  }
-}
+// Blocks to an SM that the kernels' registers are cut for, by the elements that a thread keeps of a tensor: forward 1024 threads of
+// 64 registers, half as many with more than eight elements; backward 512 threads of 128.
+constexpr int forward_blocks(int team, int elements) { return (elements > 8 ? 512 : 1024) / block_of(team); }
+constexpr int gradient_blocks(int team) { return 512 / block_of(team); }
 
-template <typename T, int V, int TEAM, int NP>
-__global__ void __launch_bounds__(block_of(TEAM)) residual_norm_kernel(const NormArgs a) {
+// LAYER: at least one of the norms is a layer norm, or there is a beta.
+template <typename T, int V, int TEAM, int NP, bool LAYER>
+__global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) residual_norm_kernel(const NormArgs a) {
   overlap_wait();
   constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM;
   __shared__ float2 slots[2 * (TEAM > 32 ? TEAM / 32 : 1)];
@@ -144,17 +125,38 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_kernel(const Nor
     at[p] = (t + p * TEAM) * V;
     live[p] = at[p] < a.channels;
   }
-  Piece<T, V> post_gamma[NP], post_beta[NP], pre_gamma[NP], pre_beta[NP];
-  load_vector<T, V, NP>(a.post_gamma, 1.f, live, at, post_gamma);
-  load_vector<T, V, NP>(a.post_beta, 0.f, live, at, post_beta);
-  load_vector<T, V, NP>(a.pre_gamma, 1.f, live, at, pre_gamma);
-  load_vector<T, V, NP>(a.pre_beta, 0.f, live, at, pre_beta);
-  float gate[NP][V];
+  // by column: scale * act(gate) * gamma and * beta of the norm behind the block; gamma and beta of the one before the next
+  float slope[NP][V], offset[NP][LAYER ? V : 1], pre_gamma[NP][V], pre_beta[NP][LAYER ? V : 1];
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+  for (int p = 0; p < NP; ++p) {
+    Piece<T, V> g, b;
+    if (live[p] && a.pre_gamma != nullptr) g.load(static_cast<const T*>(a.pre_gamma) + at[p]);
+    if (LAYER && live[p] && a.pre_beta != nullptr) b.load(static_cast<const T*>(a.pre_beta) + at[p]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) gate[p][i] = a.scale;
+    for (int i = 0; i < V; ++i) {
+      pre_gamma[p][i] = a.pre_gamma == nullptr ? 1.f : live[p] ? g.get(i) : 0.f;
+      if constexpr (LAYER) pre_beta[p][i] = a.pre_beta == nullptr || !live[p] ? 0.f : b.get(i);
+    }
+  }
   int group = -1;
+  auto enter_group = [&](int to) {
+    group = to;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      Piece<T, V> k, g, b;
+      if (live[p] && a.gate != nullptr) k.load(static_cast<const T*>(a.gate) + (size_t)group * a.channels + at[p]);
+      if (live[p] && a.post_gamma != nullptr) g.load(static_cast<const T*>(a.post_gamma) + at[p]);
+      if (LAYER && live[p] && a.post_beta != nullptr) b.load(static_cast<const T*>(a.post_beta) + at[p]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float v = a.scale;
+        if (live[p] && a.gate != nullptr) v *= activate(a.gate_activation, k.get(i));
+        if constexpr (LAYER) offset[p][i] = live[p] && a.post_beta != nullptr ? v * b.get(i) : 0.f;
+        if (live[p] && a.post_gamma != nullptr) v *= g.get(i);
+        slope[p][i] = live[p] ? v : 0.f;
+      }
+    }
+  };
 
   const T *branch = static_cast<const T*>(a.branch), *residual = static_cast<const T*>(a.residual);
   Piece<T, V> next_f[NP], next_x[NP];
@@ -167,36 +169,42 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_kernel(const Nor
         if (residual != nullptr) next_x[p].load(residual + base + at[p]);
       }
   };
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {  // (what is never loaded is zero)
+      next_f[p].set(i, 0.f);
+      next_x[p].set(i, 0.f);
+    }
   if (first < last) request(first);
+  int group_ends = first;  // the first row of the next group
+#pragma unroll 1
   for (int row = first; row < last; ++row) {
+    if (row == group_ends) {
+      enter_group(row / a.rows_per_group);
+      group_ends = (group + 1) * a.rows_per_group;
+    }
     float v[NP][V], x[NP][V];
 #pragma unroll
     for (int p = 0; p < NP; ++p)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[p][i] = live[p] ? next_f[p].get(i) : 0.f;
-        x[p][i] = live[p] && residual != nullptr ? next_x[p].get(i) : 0.f;
+        v[p][i] = next_f[p].get(i);
+        x[p][i] = next_x[p].get(i);
       }
     if (row + 1 < last) request(row + 1);
-    if (a.gate != nullptr && row / a.rows_per_group != group) {
-      group = row / a.rows_per_group;
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        if (live[p]) {
-          Piece<T, V> g;
-          g.load(static_cast<const T*>(a.gate) + (size_t)group * a.channels + at[p]);
-#pragma unroll
-          for (int i = 0; i < V; ++i) gate[p][i] = a.scale * activate(a.gate_activation, g.get(i));
-        }
-    }
     float mean1, r1, mean2, r2;
-    row_statistics<V, NP>(a.post_norm, v, live, a.inv_channels, a.epsilon, team_sum, mean1, r1);
+    row_statistics<V, NP, LAYER>(a.post_norm, v, live, a.inv_channels, a.epsilon, team_sum, mean1, r1);
     const size_t base = (size_t)row * a.channels;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        v[p][i] = live[p] ? x[p][i] + gate[p][i] * ((v[p][i] - mean1) * r1 * post_gamma[p].get(i) + post_beta[p].get(i)) : 0.f;
+      for (int i = 0; i < V; ++i) {
+        if constexpr (LAYER)
+          v[p][i] = x[p][i] + offset[p][i] + slope[p][i] * ((v[p][i] - mean1) * r1);
+        else
+          v[p][i] = x[p][i] + slope[p][i] * (v[p][i] * r1);
+      }
       if (live[p] && a.sum != nullptr) {
         Piece<T, V> s;
 #pragma unroll
@@ -205,13 +213,18 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_kernel(const Nor
       }
     }
     // (the statistics and the result are of the sum in 32 bits: the stored one is rounded once, and so is the result)
-    row_statistics<V, NP>(a.pre_norm, v, live, a.inv_channels, a.epsilon, team_sum, mean2, r2);
+    row_statistics<V, NP, LAYER>(a.pre_norm, v, live, a.inv_channels, a.epsilon, team_sum, mean2, r2);
 #pragma unroll
     for (int p = 0; p < NP; ++p)
       if (live[p] && a.out != nullptr) {
         Piece<T, V> o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.set(i, (v[p][i] - mean2) * r2 * pre_gamma[p].get(i) + pre_beta[p].get(i));
+        for (int i = 0; i < V; ++i) {
+          if constexpr (LAYER)
+            o.set(i, (v[p][i] - mean2) * r2 * pre_gamma[p][i] + pre_beta[p][i]);
+          else
+            o.set(i, v[p][i] * r2 * pre_gamma[p][i]);
+        }
         o.store(static_cast<T*>(a.out) + base + at[p]);
       }
     if (t == 0 && a.statistics != nullptr) {
@@ -306,11 +319,11 @@ __device__ __forceinline__ void unit_rows(const NormArgs& a, long long unit, int
   last = group * a.rows_per_group + (int)((long long)a.rows_per_group * (part + 1) / a.parts);
 }
 
-// LAYER: at least one of the norms is a layer norm, so that there are gradients of beta and sums of u.
+// LAYER: at least one of the norms is a layer norm, or there is a beta: gradients of beta, and sums of u.
 template <typename T, int V, int TEAM, int NP, bool LAYER>
-__global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residual_norm_grad_kernel(const NormArgs a) {
   overlap_wait();
-  constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM;
+  constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM, VL = LAYER ? V : 1;
   __shared__ float2 slots[2 * (TEAM > 32 ? TEAM / 32 : 1)];
   TeamSum<TEAM> team_sum{slots};
   const int t = (int)threadIdx.x % TEAM;
@@ -324,26 +337,53 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
     at[p] = (t + p * TEAM) * V;
     live[p] = at[p] < a.channels;
   }
-  Piece<T, V> post_gamma[NP], post_beta[NP], pre_gamma[NP];
-  load_vector<T, V, NP>(a.post_gamma, 1.f, live, at, post_gamma);
-  if constexpr (LAYER) load_vector<T, V, NP>(a.post_beta, 0.f, live, at, post_beta);
-  load_vector<T, V, NP>(a.pre_gamma, 1.f, live, at, pre_gamma);
-  float d_post_gamma[NP][V] = {}, d_pre_gamma[NP][V] = {}, d_post_beta[NP][V] = {}, d_pre_beta[NP][V] = {};
+  float pre_gamma[NP][V];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    Piece<T, V> g;
+    if (live[p] && a.pre_gamma != nullptr) g.load(static_cast<const T*>(a.pre_gamma) + at[p]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) pre_gamma[p][i] = a.pre_gamma == nullptr ? 1.f : live[p] ? g.get(i) : 0.f;
+  }
+  float d_pre_gamma[NP][V] = {}, d_pre_beta[NP][VL] = {};
+  float* line = a.partial != nullptr ? a.partial + (size_t)team * a.line : nullptr;
   const T *branch = static_cast<const T*>(a.branch), *sum = static_cast<const T*>(a.residual);
   const T *sum_grad = static_cast<const T*>(a.sum_grad), *out_grad = static_cast<const T*>(a.out_grad);
 
+#pragma unroll 1
   for (long long unit = team; unit < units; unit += teams) {
     int group, part, first, last;
     unit_rows(a, unit, group, part, first, last);
-    float gate[NP][V], d_gate[NP][V] = {};
+    // by column: scale * act(gate) * gamma, what takes the sum's gradient to u; sums over the stretch's rows of ds * hat and ds
+    float slope[NP][V], p_sum[NP][V] = {}, q_sum[NP][VL] = {};
+    auto column = [&](int p, float (&gate)[V], float (&gamma)[V]) {
+      Piece<T, V> k, g;
+      if (live[p] && a.gate != nullptr) k.load(static_cast<const T*>(a.gate) + (size_t)group * a.channels + at[p]);
+      if (live[p] && a.post_gamma != nullptr) g.load(static_cast<const T*>(a.post_gamma) + at[p]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        gate[i] = live[p] && a.gate != nullptr ? k.get(i) : 1.f;
+        gamma[i] = live[p] && a.post_gamma != nullptr ? g.get(i) : 1.f;
+      }
+    };
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      Piece<T, V> g;
-      if (a.gate != nullptr && live[p]) g.load(static_cast<const T*>(a.gate) + (size_t)group * a.channels + at[p]);
+      float gate[V], gamma[V];
+      column(p, gate, gamma);
 #pragma unroll
-      for (int i = 0; i < V; ++i) gate[p][i] = a.gate != nullptr && live[p] ? activate(a.gate_activation, g.get(i)) : 1.f;
+      for (int i = 0; i < V; ++i)
+        slope[p][i] = live[p] ? a.scale * (a.gate != nullptr ? activate(a.gate_activation, gate[i]) : 1.f) * gamma[i] : 0.f;
     }
     Piece<T, V> next_f[NP], next_s[NP], next_ds[NP], next_do[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {  // (what is never loaded is zero)
+        next_f[p].set(i, 0.f);
+        next_s[p].set(i, 0.f);
+        next_ds[p].set(i, 0.f);
+        next_do[p].set(i, 0.f);
+      }
     float next_stats[4];
     auto request = [&](int row) {
       const size_t base = (size_t)row * a.channels;
@@ -359,6 +399,7 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
       for (int i = 0; i < 4; ++i) next_stats[i] = a.statistics[(size_t)i * a.rows + row];
     };
     if (first < last) request(first);
+#pragma unroll 1
     for (int row = first; row < last; ++row) {
       const float mean1 = next_stats[0], r1 = next_stats[1], mean2 = next_stats[2], r2 = next_stats[3];
       float u[NP][V], hat[NP][V], f[NP][V], ds[NP][V];
@@ -367,15 +408,17 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
       for (int p = 0; p < NP; ++p)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float g = live[p] ? next_do[p].get(i) : 0.f;
-          hat[p][i] = live[p] ? (next_s[p].get(i) - mean2) * r2 : 0.f;
-          f[p][i] = live[p] ? (next_f[p].get(i) - mean1) * r1 : 0.f;
-          ds[p][i] = live[p] && sum_grad != nullptr ? next_ds[p].get(i) : 0.f;
-          u[p][i] = g * pre_gamma[p].get(i);
+          const float g = next_do[p].get(i);
+          hat[p][i] = LAYER ? (live[p] ? (next_s[p].get(i) - mean2) * r2 : 0.f) : next_s[p].get(i) * r2;
+          f[p][i] = LAYER ? (live[p] ? (next_f[p].get(i) - mean1) * r1 : 0.f) : next_f[p].get(i) * r1;
+          ds[p][i] = next_ds[p].get(i);
+          u[p][i] = g * pre_gamma[p][i];
           d_pre_gamma[p][i] += g * hat[p][i];
-          if constexpr (LAYER) d_pre_beta[p][i] += g;
           a1 += u[p][i] * hat[p][i];
-          if constexpr (LAYER) a2 += u[p][i];
+          if constexpr (LAYER) {
+            d_pre_beta[p][i] += g;
+            a2 += u[p][i];
+          }
         }
       if (row + 1 < last) request(row + 1);
       const size_t base = (size_t)row * a.channels;
@@ -390,7 +433,7 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) ds[p][i] += r2 * (u[p][i] - hat[p][i] * a1 - a2);
+        for (int i = 0; i < V; ++i) ds[p][i] += r2 * (LAYER ? u[p][i] - hat[p][i] * a1 - a2 : u[p][i] - hat[p][i] * a1);
         if (live[p] && a.residual_grad != nullptr) {
           Piece<T, V> o;
 #pragma unroll
@@ -399,16 +442,13 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = ds[p][i] * a.scale;
-          float n = f[p][i] * post_gamma[p].get(i);
-          if constexpr (LAYER) n += post_beta[p].get(i);
-          d_gate[p][i] += d * n;
-          const float dn = d * gate[p][i];
-          d_post_gamma[p][i] += dn * f[p][i];
-          if constexpr (LAYER) d_post_beta[p][i] += dn;
-          u[p][i] = live[p] ? dn * post_gamma[p].get(i) : 0.f;
+          p_sum[p][i] += ds[p][i] * f[p][i];
+          u[p][i] = ds[p][i] * slope[p][i];
           b1 += u[p][i] * f[p][i];
-          if constexpr (LAYER) b2 += u[p][i];
+          if constexpr (LAYER) {
+            q_sum[p][i] += ds[p][i];
+            b2 += u[p][i];
+          }
         }
       }
       if (a.post_norm != PDNN_NORM_NONE) {
@@ -423,47 +463,66 @@ __global__ void __launch_bounds__(block_of(TEAM)) residual_norm_grad_kernel(cons
         if (live[p] && a.branch_grad != nullptr) {
           Piece<T, V> o;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o.set(i, r1 * (u[p][i] - f[p][i] * b1 - b2));
+          for (int i = 0; i < V; ++i) o.set(i, r1 * (LAYER ? u[p][i] - f[p][i] * b1 - b2 : u[p][i] - f[p][i] * b1));
           o.store(static_cast<T*>(a.branch_grad) + base + at[p]);
         }
     }
-    if (a.gate_grad != nullptr) {
+    // what the stretch's sums are worth
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
-        if (live[p]) {
-          if (a.parts == 1) {
-            Piece<T, V> g, o;
-            g.load(static_cast<const T*>(a.gate) + (size_t)group * a.channels + at[p]);
+    for (int p = 0; p < NP; ++p) {
+      float gate[V], gamma[V], d_gate[V];
+      column(p, gate, gamma);
+      Piece<T, V> b;
+      if (LAYER && live[p] && a.post_beta != nullptr) b.load(static_cast<const T*>(a.post_beta) + at[p]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.set(i, d_gate[p][i] * activation_slope(a.gate_activation, g.get(i)));
-            o.store(static_cast<T*>(a.gate_grad) + (size_t)group * a.channels + at[p]);
-          } else {
-            float* to = a.gate_partial + ((size_t)part * groups + group) * a.channels + at[p];
-#pragma unroll
-            for (int i = 0; i < V; ++i) to[i] = d_gate[p][i];
-          }
+      for (int i = 0; i < V; ++i) {
+        const float k = a.scale * (a.gate != nullptr ? activate(a.gate_activation, gate[i]) : 1.f);
+        // (the line takes the sums over a team's stretches, most often one: registers for them are needed elsewhere)
+        if (live[p] && line != nullptr && a.slot[0] >= 0) {
+          float* to = line + (size_t)a.slot[0] * a.channels + at[p] + i;
+          *to = (unit == team ? 0.f : *to) + k * p_sum[p][i];
         }
+        d_gate[i] = gamma[i] * p_sum[p][i];
+        if constexpr (LAYER) {
+          if (live[p] && line != nullptr && a.slot[1] >= 0) {
+            float* to = line + (size_t)a.slot[1] * a.channels + at[p] + i;
+            *to = (unit == team ? 0.f : *to) + k * q_sum[p][i];
+          }
+          if (live[p] && a.post_beta != nullptr) d_gate[i] += b.get(i) * q_sum[p][i];
+        }
+        d_gate[i] *= a.scale;
+      }
+      if (a.gate_grad == nullptr || !live[p]) continue;
+      if (a.parts == 1) {
+        Piece<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.set(i, d_gate[i] * activation_slope(a.gate_activation, gate[i]));
+        o.store(static_cast<T*>(a.gate_grad) + (size_t)group * a.channels + at[p]);
+      } else {
+        float* to = a.gate_partial + (size_t)part * a.gate_line + (size_t)group * a.channels + at[p];
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = d_gate[i];
+      }
     }
   }
-  if (a.partial != nullptr) {
-    float* line = a.partial + (size_t)team * a.vectors * a.channels;
+  if (line == nullptr) return;
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-      if (live[p]) {
+  for (int p = 0; p < NP; ++p) {
+    if (!live[p]) continue;
+    for (int which = 0; which < 2; ++which)  // a team without rows
+      if (team >= units && a.slot[which] >= 0)
+        for (int i = 0; i < V; ++i) line[(size_t)a.slot[which] * a.channels + at[p] + i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (a.slot[0] >= 0) line[(size_t)a.slot[0] * a.channels + at[p] + i] = d_post_gamma[p][i];
-          if (a.slot[2] >= 0) line[(size_t)a.slot[2] * a.channels + at[p] + i] = d_pre_gamma[p][i];
-          if constexpr (LAYER) {
-            if (a.slot[1] >= 0) line[(size_t)a.slot[1] * a.channels + at[p] + i] = d_post_beta[p][i];
-            if (a.slot[3] >= 0) line[(size_t)a.slot[3] * a.channels + at[p] + i] = d_pre_beta[p][i];
-          }
-        }
+    for (int i = 0; i < V; ++i) {
+      if (a.slot[2] >= 0) line[(size_t)a.slot[2] * a.channels + at[p] + i] = d_pre_gamma[p][i];
+      if constexpr (LAYER) {
+        if (a.slot[3] >= 0) line[(size_t)a.slot[3] * a.channels + at[p] + i] = d_pre_beta[p][i];
       }
+    }
   }
 }
 
-// Rows that no team can keep: a block walks its row four times, and the partial sums over rows are lines in memory that
+// Rows that no team can keep: a block walks its row three times, and the partial sums over rows are lines in memory that
 // the block adds to (nobody else touches them).
 template <typename T>
 __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const NormArgs a) {
@@ -474,15 +533,15 @@ __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const Nor
   const long long units = (long long)groups * a.parts;
   const T *branch = static_cast<const T*>(a.branch), *sum = static_cast<const T*>(a.residual);
   const T *sum_grad = static_cast<const T*>(a.sum_grad), *out_grad = static_cast<const T*>(a.out_grad);
-  float* line = a.partial != nullptr ? a.partial + (size_t)blockIdx.x * a.vectors * a.channels : nullptr;
+  float* line = a.partial != nullptr ? a.partial + (size_t)blockIdx.x * a.line : nullptr;
   if (line != nullptr)
     for (int c = (int)threadIdx.x; c < a.channels; c += 1024)
-      for (int k = 0; k < a.vectors; ++k) line[(size_t)k * a.channels + c] = 0.f;
+      for (size_t k = c; k < a.line; k += a.channels) line[k] = 0.f;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
     int group, part, first, last;
     unit_rows(a, unit, group, part, first, last);
     const T* gate = a.gate != nullptr ? static_cast<const T*>(a.gate) + (size_t)group * a.channels : nullptr;
-    float* gate_line = a.gate_partial != nullptr ? a.gate_partial + ((size_t)part * groups + group) * a.channels : nullptr;
+    float* gate_line = a.gate_partial != nullptr ? a.gate_partial + (size_t)part * a.gate_line + (size_t)group * a.channels : nullptr;
     if (gate_line != nullptr)
       for (int c = (int)threadIdx.x; c < a.channels; c += 1024) gate_line[c] = 0.f;
     for (int row = first; row < last; ++row) {
@@ -546,11 +605,17 @@ __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const Nor
 // What becomes of the sums over rows.
 template <typename T>
 struct StoreVectors {
-  T* to[4];
-  int channels;
+  T* to[5];
+  const T* gate;  // of vector gate_vector
+  int channels, gate_vector, activation;
   __device__ __forceinline__ void operator()(size_t i, float sum) const {
-    const int which = (int)(i / channels);
-    to[which][i % channels] = from_f32<T>(sum);
+    const int which = (int)(i / channels), c = (int)(i - (size_t)which * channels);
+    if (which == gate_vector) sum *= activation_slope(activation, to_f32(gate[c]));
+    T* p = to[0];
+#pragma unroll
+    for (int v = 1; v < 5; ++v)
+      if (which == v) p = to[v];
+    p[c] = from_f32<T>(sum);
   }
 };
 template <typename T>
@@ -578,24 +643,30 @@ struct Shape {
   static constexpr int team = TEAM, np = NP;
 };
 
-// The smallest team that keeps a row of `pieces` packets or elements; 0 where none does.
-template <typename F>
-int with_shape(bool packets, int pieces, F&& f) {
-  if (packets) {
+// The smallest team that keeps a row of `pieces` packets (PACKETS) or elements; 0 where none does.
+template <bool PACKETS, typename F>
+int with_shape(int pieces, F&& f) {
+  if constexpr (PACKETS) {
     if (pieces <= 32) return f(Shape<32, 1>{});
-    if (pieces <= 64) return f(Shape<32, 2>{});
+    if (pieces <= 64) return f(Shape<64, 1>{});
     if (pieces <= 128) return f(Shape<128, 1>{});
     if (pieces <= 256) return f(Shape<256, 1>{});
     if (pieces <= 512) return f(Shape<512, 1>{});
     if (pieces <= 1024) return f(Shape<512, 2>{});
-    return 0;
+  } else {
+    if (pieces <= 128) return f(Shape<32, 4>{});
+    if (pieces <= 512) return f(Shape<128, 4>{});
+    if (pieces <= 1024) return f(Shape<256, 4>{});
+    if (pieces <= 2048) return f(Shape<512, 4>{});
+    if (pieces <= 4096) return f(Shape<512, 8>{});
   }
-  if (pieces <= 128) return f(Shape<32, 4>{});
-  if (pieces <= 512) return f(Shape<128, 4>{});
-  if (pieces <= 1024) return f(Shape<256, 4>{});
-  if (pieces <= 2048) return f(Shape<512, 4>{});
-  if (pieces <= 4096) return f(Shape<512, 8>{});
   return 0;
+}
+template <typename T, typename F>
+int with_pieces(bool packets, int channels, F&& f) {
+  constexpr int N = Vec16<T>::N;
+  if (packets) return with_shape<true>(channels / N, [&](auto shape) { return f(std::integral_constant<int, N>{}, shape); });
+  return with_shape<false>(channels, [&](auto shape) { return f(std::integral_constant<int, 1>{}, shape); });
 }
 
 int check_params(const char* what, int dtype, const PdnnResidualNormParams& p) {
@@ -657,21 +728,21 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
   a.sum = t.sum;
   a.out = t.output;
   a.statistics = t.statistics;
+  const bool layer = p.post_norm == PDNN_NORM_LAYER || p.pre_norm == PDNN_NORM_LAYER || t.post_beta != nullptr || t.pre_beta != nullptr;
   return dispatch(dtype, [&](auto type) {
     using T = decltype(type);
     constexpr int N = Vec16<T>::N;
     const bool packets = p.channels % N == 0 && all_aligned({t.branch, t.residual, t.post_gamma, t.post_beta, t.gate,
                                                              t.pre_gamma, t.pre_beta, t.sum, t.output});
-    const int pieces = packets ? p.channels / N : p.channels;
-    const int known = with_shape(packets, pieces, [&](auto shape) {
-      constexpr int TEAM = decltype(shape)::team, NP = decltype(shape)::np, kTeams = block_of(TEAM) / TEAM;
-      // (as many teams as the device holds at 64 registers a thread or so, with a row or more to each)
-      const long long wave = (long long)sms * std::max(1024 / block_of(TEAM), 1);
+    const int known = with_pieces<T>(packets, p.channels, [&](auto width, auto shape) {
+      constexpr int V = decltype(width)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np, kTeams = block_of(TEAM) / TEAM;
+      // one wave, with a row or more to each team
+      const long long wave = (long long)sms * forward_blocks(TEAM, V * NP);
       const unsigned grid = (unsigned)std::min<long long>(wave, ((long long)p.rows + kTeams - 1) / kTeams);
-      if (packets)
-        launch_overlapped(residual_norm_kernel<T, N, TEAM, NP>, grid, block_of(TEAM), s, a);
+      if (layer)
+        launch_overlapped(residual_norm_kernel<T, V, TEAM, NP, true>, grid, block_of(TEAM), s, a);
       else
-        launch_overlapped(residual_norm_kernel<T, 1, TEAM, NP>, grid, block_of(TEAM), s, a);
+        launch_overlapped(residual_norm_kernel<T, V, TEAM, NP, false>, grid, block_of(TEAM), s, a);
       return 1;
     });
     if (known == 0) {
@@ -728,43 +799,44 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
     const bool packets = p.channels % N == 0 &&
                          all_aligned({t.branch, t.sum, t.post_gamma, t.post_beta, t.gate, t.pre_gamma, g.sum_grad, g.output_grad,
                                       g.branch_grad, g.residual_grad, g.gate_grad});
-    const int pieces = packets ? p.channels / N : p.channels, groups = p.rows / a.rows_per_group;
+    const int groups = p.rows / a.rows_per_group;
     // The cut of the groups for at most `wave` teams, and scratch for what the teams leave: a line to a team of the grid (of
     // which a block has `to_block`) and one to a group's part.  Returns the blocks, 0 where there is no scratch.
     void* scratch = nullptr;
     long long teams = 0;
+    bool joined = false;  // the gate's sums are a vector of the teams' lines
     auto plan = [&](long long wave, int to_block, bool direct) {
       a.parts = (int)std::max<long long>(1, std::min<long long>(wave / groups, a.rows_per_group));
       const long long blocks = (std::min<long long>(wave, (long long)groups * a.parts) + to_block - 1) / to_block;
       teams = blocks * to_block;
-      const size_t lines = a.vectors > 0 ? (size_t)teams * a.vectors * p.channels : 0;
-      const size_t gates = g.gate_grad != nullptr && !(direct && a.parts == 1) ? (size_t)groups * a.parts * p.channels : 0;
-      if (lines + gates > 0) {
-        if (cudaMallocAsync(&scratch, (lines + gates) * sizeof(float), s) != cudaSuccess) {
+      const bool gates = g.gate_grad != nullptr && !(direct && a.parts == 1);
+      // (the parts of one group are the teams, but for teams without rows: their vector of the line is then not added)
+      joined = gates && groups == 1 && teams == a.parts;
+      a.line = (size_t)(a.vectors + (joined ? 1 : 0)) * p.channels;
+      const size_t lines = (size_t)teams * a.line, apart = gates && !joined ? (size_t)groups * a.parts * p.channels : 0;
+      if (lines + apart > 0) {
+        if (cudaMallocAsync(&scratch, (lines + apart) * sizeof(float), s) != cudaSuccess) {
           cudaGetLastError();
           scratch = nullptr;
           return 0u;
         }
         a.partial = lines > 0 ? static_cast<float*>(scratch) : nullptr;
-        a.gate_partial = gates > 0 ? static_cast<float*>(scratch) + lines : nullptr;
+        if (gates) a.gate_partial = static_cast<float*>(scratch) + (joined ? (size_t)a.vectors * p.channels : lines);
+        a.gate_line = joined ? a.line : (size_t)groups * p.channels;
       }
       return (unsigned)blocks;
     };
     unsigned grid = 0;
-    const int known = with_shape(packets, pieces, [&](auto shape) {
-      constexpr int TEAM = decltype(shape)::team, NP = decltype(shape)::np, kThreads = block_of(TEAM), kTeams = kThreads / TEAM;
-      // One block of 512 threads to an SM (its sums and the next row take most of the registers), or as many threads.
-      const long long wave = std::min<long long>((long long)sms * std::max(512 / kThreads, 1) * kTeams, p.rows);
+    const int known = with_pieces<T>(packets, p.channels, [&](auto width, auto shape) {
+      constexpr int V = decltype(width)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np;
+      constexpr int kThreads = block_of(TEAM), kTeams = kThreads / TEAM;
+      const long long wave = std::min<long long>((long long)sms * gradient_blocks(TEAM) * kTeams, p.rows);
       grid = plan(wave, kTeams, true);
       if (grid == 0) return 1;
-      if (packets && layer)
-        launch_overlapped(residual_norm_grad_kernel<T, N, TEAM, NP, true>, grid, kThreads, s, a);
-      else if (packets)
-        launch_overlapped(residual_norm_grad_kernel<T, N, TEAM, NP, false>, grid, kThreads, s, a);
-      else if (layer)
-        launch_overlapped(residual_norm_grad_kernel<T, 1, TEAM, NP, true>, grid, kThreads, s, a);
+      if (layer)
+        launch_overlapped(residual_norm_grad_kernel<T, V, TEAM, NP, true>, grid, kThreads, s, a);
       else
-        launch_overlapped(residual_norm_grad_kernel<T, 1, TEAM, NP, false>, grid, kThreads, s, a);
+        launch_overlapped(residual_norm_grad_kernel<T, V, TEAM, NP, false>, grid, kThreads, s, a);
       return 1;
     });
     if (known == 0) {
@@ -776,12 +848,16 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
     if (status == PDNN_OK && a.partial != nullptr) {
       StoreVectors<T> store;
       store.channels = p.channels;
+      store.gate = joined ? static_cast<const T*>(t.gate) : nullptr;
+      store.gate_vector = joined ? a.vectors : -1;
+      store.activation = p.gate_activation;
       for (int i = 0; i < 4; ++i)
         if (a.slot[i] >= 0) store.to[a.slot[i]] = static_cast<T*>(vectors[i]);
-      launch_column_sums(a.partial, (int)teams, (size_t)a.vectors * p.channels, sms, s, store);
+      if (joined) store.to[a.vectors] = static_cast<T*>(g.gate_grad);
+      launch_column_sums(a.partial, (int)teams, a.line, sms, s, store);
       status = check_launch(what);
     }
-    if (status == PDNN_OK && a.gate_partial != nullptr) {
+    if (status == PDNN_OK && a.gate_partial != nullptr && !joined) {
       launch_column_sums(a.gate_partial, a.parts, (size_t)groups * p.channels, sms, s,
                          StoreGate<T>{static_cast<T*>(g.gate_grad), static_cast<const T*>(t.gate), p.gate_activation});
       status = check_launch(what);
