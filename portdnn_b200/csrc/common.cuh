@@ -78,21 +78,52 @@ __device__ __forceinline__ void store16(T* p, const Vec16<T>& v) {
   *reinterpret_cast<uint4*>(p) = v.raw;
 }
 
-// V elements as a thread keeps them: a 16-byte packet or a single element.
+// Two neighbouring elements as one word, rounded (16-bit types).
+template <typename T>
+__device__ __forceinline__ uint32_t pair_word(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pair_word<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pair_word<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// V elements as a thread keeps them: a 16-byte packet, a pair of 16-bit elements or a single element.
 template <typename T, int V>
 struct Piece {
   Vec16<T> raw;
   __device__ __forceinline__ void load(const T* p) { raw = load16(p); }
   __device__ __forceinline__ float get(int i) const { return to_f32(raw.get(i)); }
-  __device__ __forceinline__ void set(int i, float v) { raw.set(i, from_f32<T>(v)); }
+  __device__ __forceinline__ void clear() { raw.raw = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void round(const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+      raw.raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+      raw.raw = make_uint4(pair_word<T>(v[0], v[1]), pair_word<T>(v[2], v[3]), pair_word<T>(v[4], v[5]), pair_word<T>(v[6], v[7]));
+    }
+  }
   __device__ __forceinline__ void store(T* p) const { store16(p, raw); }
+};
+template <typename T>
+struct Piece<T, 2> {
+  uint32_t raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(&raw)[i]); }
+  __device__ __forceinline__ void clear() { raw = 0u; }
+  __device__ __forceinline__ void round(const float (&v)[2]) { raw = pair_word<T>(v[0], v[1]); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint32_t*>(p) = raw; }
 };
 template <typename T>
 struct Piece<T, 1> {
   T raw;
   __device__ __forceinline__ void load(const T* p) { raw = *p; }
   __device__ __forceinline__ float get(int) const { return to_f32(raw); }
-  __device__ __forceinline__ void set(int, float v) { raw = from_f32<T>(v); }
+  __device__ __forceinline__ void clear() { raw = from_f32<T>(0.f); }
+  __device__ __forceinline__ void round(const float (&v)[1]) { raw = from_f32<T>(v[0]); }
   __device__ __forceinline__ void store(T* p) const { *p = raw; }
 };
 

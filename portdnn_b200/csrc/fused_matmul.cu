@@ -121,19 +121,19 @@ __global__ void __launch_bounds__(32 * kSlopeLanes) activation_slope_kernel(cons
         for (int u = 0; u < kAhead; ++u) {
           const int r = r0 + u * kSlopeLanes;
           if (r >= last) continue;
-          Piece<T, V> o;
+          float dz[V];
 #pragma unroll
           for (int i = 0; i < V; i += 2) {
             constexpr int kNext = V > 1 ? 1 : 0;
             float2 v = make_float2(a.scale * d[u].get(i), a.scale * d[u].get(i + kNext));
             if (ACT != PDNN_ACT_NONE) v = mul2(v, slope_of<ACT, T>(make_float2(z[u].get(i), z[u].get(i + kNext))));
-            o.set(i, v.x);
-            sum[i] += v.x;
-            if (V > 1) {
-              o.set(i + kNext, v.y);
-              sum[i + kNext] += v.y;
-            }
+            dz[i + kNext] = v.y;
+            dz[i] = v.x;
           }
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] += dz[i];
+          Piece<T, V> o;
+          o.round(dz);
           if (a.dz != nullptr) o.store(static_cast<T*>(a.dz) + (long long)r * a.dz_pitch + col);
         }
       }

@@ -35,7 +35,7 @@ struct LossArgs {
   const float *advantages, *old_logp, *ref_logp, *weights;
   float *token_loss, *logp;
   void* grad;
-  int rows, vocab, wide_targets, packets;
+  int rows, vocab, wide_targets;
   long long pitch, grad_pitch;
   float c, inv_temperature, clip_low, clip_high, kl, grad_scale;  // c = log2(e) / temperature
 };
@@ -56,23 +56,11 @@ __device__ __forceinline__ void store_streaming(T* p, const Vec16<T>& v) {
   __stcs(reinterpret_cast<uint4*>(p), v.raw);
 }
 
-// Two neighbouring results as one word, rounded.
-template <typename T>
-__device__ __forceinline__ uint32_t pair_word(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 // One row to a cluster of CTAs (most often to a CTA).  An element costs an exponential in either walk, and as little else as
 // possible: product and shift are one multiply-add, the gradient's factor is added to the exponent and its sign put
 // on afterwards, and the chosen token's entry is written over at the end.
 template <typename T>
-__global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
+__global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
   overlap_wait();
   constexpr int N = Vec16<T>::N, kUnroll = 4;
   __shared__ Partial warp_part[16];
@@ -85,10 +73,23 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
   const int row = (int)(blockIdx.x / ranks);
   const T* x = static_cast<const T*>(a.logits) + (size_t)row * a.pitch;
   T* g = a.grad != nullptr ? static_cast<T*>(a.grad) + (size_t)row * a.grad_pitch : nullptr;
-  // this CTA's share of the row, whole packets but for the end
+  // this CTA's share of the row: [begin, body) and [tail, end) are what lies in front of the first 16-byte boundary and behind
+  // the last; where logits and gradient lie on different ones there are no packets
   const int share = ((a.vocab + (int)ranks - 1) / (int)ranks + N - 1) / N * N;
   const int begin = min((int)rank * share, a.vocab), end = min(begin + share, a.vocab);
-  const int packed_end = a.packets ? begin + (end - begin) / N * N : begin;
+  const int head = (int)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) & 15) / (int)sizeof(T);
+  const bool packets = g == nullptr || ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+  const int body = packets ? min(begin + head, end) : end, tail = packets ? body + (end - body) / N * N : end;
+  const int kStep = threads * N;
+  // f(whole, j): the packets at j, j + kStep, .. of the body, kUnroll of them, or as many as there are where it is not whole;
+  // single(j): an element around it
+  auto walk = [&](auto&& f, auto&& single) {
+    int j = body + tid * N;
+    for (; j + (kUnroll - 1) * kStep < tail; j += kUnroll * kStep) f(std::true_type{}, j);
+    if (j < tail) f(std::false_type{}, j);
+    for (j = begin + tid; j < body; j += threads) single(j);
+    for (j = tail + tid; j < end; j += threads) single(j);
+  };
   const long long t = a.wide_targets ? static_cast<const long long*>(a.targets)[row] : (long long)static_cast<const int*>(a.targets)[row];
   const float weight = a.weights != nullptr ? a.weights[row] : 1.f;
   // A row without weight or without a token counts for nothing, whatever stands in it: it is not read.
@@ -101,8 +102,11 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
     if (g != nullptr) {
       Vec16<T> zero;
       zero.raw = make_uint4(0u, 0u, 0u, 0u);
-      for (int j = begin + tid * N; j < packed_end; j += threads * N) store_streaming(g + j, zero);
-      for (int j = packed_end + tid; j < end; j += threads) g[j] = from_f32<T>(0.f);
+      walk([&](auto whole, int j) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (whole || j + u * kStep < tail) store_streaming(g + j + u * kStep, zero);
+      }, [&](int j) { g[j] = from_f32<T>(0.f); });
     }
     return;  // (all CTAs of the cluster alike)
   }
@@ -133,21 +137,18 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
     for (int i = 0; i < N; ++i) v[i] = to_f32(p.get(i));
     take(v, N);
   };
-  {
-    int j = begin + tid * N;
-    for (; j + (kUnroll - 1) * threads * N < packed_end; j += kUnroll * threads * N) {
-      Vec16<T> p[kUnroll];
+  walk([&](auto whole, int j) {
+    Vec16<T> p[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * threads * N);
+    for (int u = 0; u < kUnroll; ++u)
+      if (whole || j + u * kStep < tail) p[u] = load16(x + j + u * kStep);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) take_packet(p[u]);
-    }
-    for (; j < packed_end; j += threads * N) take_packet(load16(x + j));
-    for (int k = packed_end + tid; k < end; k += threads) {
-      const float v = to_f32(x[k]);
-      take(&v, 1);
-    }
-  }
+    for (int u = 0; u < kUnroll; ++u)
+      if (whole || j + u * kStep < tail) take_packet(p[u]);
+  }, [&](int j) {
+    const float v = to_f32(x[j]);
+    take(&v, 1);
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Partial other{__shfl_xor_sync(0xFFFFFFFFu, part.shift, o), __shfl_xor_sync(0xFFFFFFFFu, part.sum, o)};
@@ -219,27 +220,23 @@ __global__ void __launch_bounds__(512) policy_loss_kernel(const LossArgs a) {
     }
     return o;
   };
-  const int kStep = threads * N;
-  if (none) {
-    Vec16<T> zero;
-    zero.raw = make_uint4(0u, 0u, 0u, 0u);
-    for (int j = begin + tid * N; j < packed_end; j += kStep) store_streaming(g + j, zero);
-    for (int j = packed_end + tid; j < end; j += threads) g[j] = from_f32<T>(0.f);
-  } else {
-    int j = begin + tid * N;
-    for (; j + (kUnroll - 1) * kStep < packed_end; j += kUnroll * kStep) {
-      Vec16<T> p[kUnroll];
+  auto alone = [&](int j) {
+    const float e = exp2_fast(fmaf(to_f32(x[j]), a.c, lift));
+    g[j] = from_f32<T>(none ? 0.f : slope > 0.f ? -e : e);
+  };
+  walk([&](auto whole, int j) {
+    Vec16<T> p[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) p[u] = load16(x + j + u * kStep);
+    for (int u = 0; u < kUnroll; ++u)
+      if (whole || j + u * kStep < tail) p[u] = load16(x + j + u * kStep);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) store_streaming(g + j + u * kStep, packet(p[u]));
-    }
-    for (; j < packed_end; j += kStep) store_streaming(g + j, packet(load16(x + j)));
-    for (int j1 = packed_end + tid; j1 < end; j1 += threads) {
-      const float e = exp2_fast(fmaf(to_f32(x[j1]), a.c, lift));
-      g[j1] = from_f32<T>(slope > 0.f ? -e : e);
-    }
-  }
+    for (int u = 0; u < kUnroll; ++u)
+      if (whole || j + u * kStep < tail) {
+        Vec16<T> o = packet(p[u]);
+        if (none) o.raw = make_uint4(0u, 0u, 0u, 0u);
+        store_streaming(g + j + u * kStep, o);
+      }
+  }, alone);
   __syncthreads();
   if (tid == 0 && t >= begin && t < end) g[t] = from_f32<T>(chosen_grad);
 }
@@ -322,8 +319,6 @@ int launch_policy_loss(int dtype, const PdnnPolicyLossParams& p, const PdnnPolic
     a.wide_targets = p.target_bytes == 8;
     a.pitch = p.logits_pitch;
     a.grad_pitch = p.grad_pitch;
-    a.packets = aligned16(t.logits) && p.logits_pitch * es % 16 == 0 &&
-                (t.grad == nullptr || (aligned16(t.grad) && p.grad_pitch * es % 16 == 0));
     a.inv_temperature = 1.f / p.temperature;
     a.c = kLog2e / p.temperature;
     a.clip_low = p.clip_low;
@@ -335,8 +330,10 @@ int launch_policy_loss(int dtype, const PdnnPolicyLossParams& p, const PdnnPolic
     const long long packets = ((long long)p.vocab * es + 15) / 16;
     int cluster = 1;
     while (cluster < 8 && (long long)p.rows * cluster * 2 <= 2ll * sms && packets / (cluster * 2) >= 128) cluster *= 2;
-    int threads = 128;
-    while (threads < 512 && packets / cluster > 2 * threads) threads *= 2;
+    // (rows enough for many blocks to an SM: four packets to a thread, so that a row's chain of latencies overlaps others)
+    const int to_thread = (long long)p.rows * cluster >= 8ll * sms ? 4 : 2;
+    int threads = to_thread == 4 ? 64 : 128;
+    while (threads < 512 && packets / cluster > to_thread * threads) threads *= 2;
     if (dtype == PDNN_F32) launch_rows<float>(a, cluster, threads, s);
     if (dtype == PDNN_F16) launch_rows<__half>(a, cluster, threads, s);
     if (dtype == PDNN_BF16) launch_rows<__nv_bfloat16>(a, cluster, threads, s);

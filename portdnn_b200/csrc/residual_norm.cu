@@ -10,7 +10,7 @@
 //
 // Bound by memory: forward reads two tensors and writes two, backward reads four and writes two, each once.  A
 // team of threads keeps a row in registers (a packet or two to a thread), so that statistics over the row - taken
-// about the mean, in fp32 - cost no second read, and requests the next row before it reduces this one.  Teams keep to
+// about the mean, in fp32 - cost no second read, and has the next three rows on their way.  Teams keep to
 // whole stretches of rows: what depends on the column alone stays in registers, multiplied out (scale * act(gate) * gamma
 // is one number), and the sums over rows of the backward pass are the thread's own until its stretch ends.  Both of
 // the gradients behind the post norm's result come of one sum over the group's rows, P = sum ds * hat: gamma's is
@@ -22,10 +22,88 @@
 #include <algorithm>
 #include <cstring>
 #include <initializer_list>
+#include <mutex>
+#include <set>
 #include <type_traits>
 
 namespace pdnn {
 namespace {
+
+// Rows on their way: a thread asks for its own pieces of the rows to come, kAhead of them, with cp.async into slots of shared
+// memory that nobody else touches, so that no barrier is needed and no registers wait.  (Packets; smaller pieces are
+// requested into registers one row ahead: four bytes to a copy are too few, 1999x1003 f32 gradient 23.4 us so, 21.9 in registers.)
+template <typename T, int V>
+constexpr bool in_slots() { return V * sizeof(T) == 16; }
+
+__device__ __forceinline__ void async_copy(void* slot, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// TENSORS tensors' pieces of a thread, NP of each, AHEAD rows.
+template <typename T, int V, int NP, int TENSORS, int AHEAD, int THREADS>
+struct Incoming {
+  static constexpr bool kSlots = in_slots<T, V>();
+  static constexpr int kBytes = V * (int)sizeof(T), kRow = TENSORS * NP * THREADS * kBytes;
+  static constexpr int kFit = 200 * 1024 / kRow, kDepth = !kSlots || kFit < 1 ? 1 : kFit < AHEAD ? kFit : AHEAD;
+  static constexpr int kSharedBytes = kSlots ? kDepth * kRow : 0;
+  Piece<T, V> held[kSlots ? 1 : TENSORS][NP];
+  char* mine;  // [depth][tensor][piece][thread]
+  int slot = 0;
+
+  __device__ __forceinline__ Incoming(char* shared) : mine(shared + (int)threadIdx.x * kBytes) {
+    Piece<T, V> zero;
+    zero.clear();
+    if constexpr (kSlots) {  // (what is never asked for is zero)
+      for (int i = 0; i < kDepth * TENSORS * NP; ++i) zero.store(reinterpret_cast<T*>(mine + i * THREADS * kBytes));
+    } else {
+#pragma unroll
+      for (int i = 0; i < TENSORS; ++i)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) held[i][p] = zero;
+    }
+  }
+  // Asks for a row's pieces (null tensors stay zero) into the slot of `row` steps from now; one group a row, asked for or not.
+  __device__ __forceinline__ void request(const T* const (&from)[TENSORS], size_t base, bool wanted, const bool (&live)[NP],
+                                          const int (&at)[NP], int into) {
+    if (wanted) {
+#pragma unroll
+      for (int i = 0; i < TENSORS; ++i)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          if (live[p] && from[i] != nullptr) {
+            if constexpr (kSlots)
+              async_copy(mine + ((into * TENSORS + i) * NP + p) * THREADS * kBytes, from[i] + base + at[p]);
+            else
+              held[i][p].load(from[i] + base + at[p]);
+          }
+    }
+    if constexpr (kSlots) async_commit();
+  }
+  // The oldest row's pieces.
+  __device__ __forceinline__ void take(Piece<T, V> (&to)[TENSORS][NP]) {
+    if constexpr (kSlots) {
+      async_wait<kDepth - 1>();
+#pragma unroll
+      for (int i = 0; i < TENSORS; ++i)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) to[i][p].load(reinterpret_cast<const T*>(mine + ((slot * TENSORS + i) * NP + p) * THREADS * kBytes));
+    } else {
+#pragma unroll
+      for (int i = 0; i < TENSORS; ++i)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) to[i][p] = held[i][p];
+    }
+  }
+  // The slot just taken from is the next one to be filled.
+  __device__ __forceinline__ int freed() {
+    const int s = slot;
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
+    return s;
+  }
+};
 
 struct NormArgs {
   const void *branch, *residual, *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
@@ -36,43 +114,53 @@ struct NormArgs {
   // backward
   const void *sum_grad, *out_grad;
   void *branch_grad, *residual_grad, *gate_grad;
-  // Partial sums: a line of `line` floats to a team, the parameter vectors' behind one another; to each part of the groups
-  // gate_line floats from gate_partial on, [groups][channels] (with one group a further vector of the same lines).
+  // Partial sums: a line of `line` floats to a block, the parameter vectors' behind one another, the gate's too (vector
+  // gate_vector) where there is one group; with more groups (gate_vector -1) the gate's are [parts][groups][channels].
   float *partial, *gate_partial;
-  size_t line, gate_line;
+  size_t line;
   int parts;    // stretches of rows that a group is cut into
   int vectors;  // parameter vectors with a gradient
+  int gate_vector;
   int slot[4];                    // where in a line of `partial` post gamma, post beta, pre gamma, pre beta are; -1: nowhere
 };
 
-// Sums over a team.  Teams of a warp need no barrier; others use two sets of slots in turn, so that one barrier a
-// reduction is enough: whoever is about to write a set has passed the barrier behind everybody's last read of it.
+// Sums over a team of one value or two.  Teams of a warp need no barrier; others use two sets of slots in turn, so that one
+// barrier a reduction is enough: whoever is about to write a set has passed the barrier behind everybody's last read of it.
+// (Each warp adds the warps' sums up in shuffles: a thread that reads all sixteen of 512 threads has as much to do with them as with
+// its eight elements.)
 template <int TEAM>
 struct TeamSum {
   float2* slots;  // [2][TEAM / 32]
   int turn = 0;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  template <int COUNT>
+  __device__ __forceinline__ float2 sum(float a, float b) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-      b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+      if (COUNT == 2) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
     }
     if constexpr (TEAM > 32) {
       constexpr int W = TEAM / 32;
       float2* mine = slots + turn * W;
       turn ^= 1;
-      if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = make_float2(a, b);
+      if ((threadIdx.x & 31) == 0) {
+        if (COUNT == 2) mine[threadIdx.x >> 5] = make_float2(a, b);
+        else mine[threadIdx.x >> 5].x = a;
+      }
       __syncthreads();
-      a = b = 0.f;
+      const int from = (int)threadIdx.x & (W - 1);
+      a = mine[from].x;
+      if (COUNT == 2) b = mine[from].y;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float2 v = mine[w];
-        a += v.x;
-        b += v.y;
+      for (int o = W / 2; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        if (COUNT == 2) b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
       }
     }
     return make_float2(a, b);
   }
+  __device__ __forceinline__ float one(float a) { return sum<1>(a, 0.f).x; }
+  __device__ __forceinline__ float2 two(float a, float b) { return sum<2>(a, b); }
 };
 
 constexpr int block_of(int team) { return team == 32 ? 256 : team; }
@@ -90,7 +178,7 @@ __device__ __forceinline__ void row_statistics(int kind, const float (&v)[NP][V]
     for (int p = 0; p < NP; ++p)
 #pragma unroll
       for (int i = 0; i < V; ++i) total += v[p][i];
-    mean = team_sum(total, 0.f).x * inv_channels;
+    mean = team_sum.one(total) * inv_channels;
   }
   float squares = 0.f;
 #pragma unroll
@@ -100,18 +188,21 @@ __device__ __forceinline__ void row_statistics(int kind, const float (&v)[NP][V]
       const float d = LAYER ? v[p][i] - mean : v[p][i];
       if (!LAYER || live[p]) squares += d * d;  // (entries that are not live are zero)
     }
-  r = 1.f / sqrtf(team_sum(squares, 0.f).x * inv_channels + epsilon);
+  r = 1.f / sqrtf(team_sum.one(squares) * inv_channels + epsilon);
 }
 
 // Blocks to an SM that the kernels' registers are cut for, by the elements that a thread keeps of a tensor: forward 1024 threads of
 // 64 registers, half as many with more than eight elements; backward 512 threads of 128.
 constexpr int forward_blocks(int team, int elements) { return (elements > 8 ? 512 : 1024) / block_of(team); }
-constexpr int gradient_blocks(int team) { return 512 / block_of(team); }
+constexpr int gradient_blocks(int team) { return team > 512 ? 1 : 512 / block_of(team); }
 
 // LAYER: at least one of the norms is a layer norm, or there is a beta.
+template <typename T, int V, int TEAM, int NP>
+using ForwardRows = Incoming<T, V, NP, 2, 3, block_of(TEAM)>;
 template <typename T, int V, int TEAM, int NP, bool LAYER>
 __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) residual_norm_kernel(const NormArgs a) {
   overlap_wait();
+  extern __shared__ __align__(16) char rows_shared[];
   constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM;
   __shared__ float2 slots[2 * (TEAM > 32 ? TEAM / 32 : 1)];
   TeamSum<TEAM> team_sum{slots};
@@ -158,25 +249,12 @@ __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) 
     }
   };
 
-  const T *branch = static_cast<const T*>(a.branch), *residual = static_cast<const T*>(a.residual);
-  Piece<T, V> next_f[NP], next_x[NP];
-  auto request = [&](int row) {
-    const size_t base = (size_t)row * a.channels;
+  using Rows = ForwardRows<T, V, TEAM, NP>;
+  Rows incoming(rows_shared);
+  const T* const from[2] = {static_cast<const T*>(a.branch), static_cast<const T*>(a.residual)};
+  auto request = [&](int row, int into) { incoming.request(from, (size_t)row * a.channels, row < last, live, at, into); };
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-      if (live[p]) {
-        next_f[p].load(branch + base + at[p]);
-        if (residual != nullptr) next_x[p].load(residual + base + at[p]);
-      }
-  };
-#pragma unroll
-  for (int p = 0; p < NP; ++p)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {  // (what is never loaded is zero)
-      next_f[p].set(i, 0.f);
-      next_x[p].set(i, 0.f);
-    }
-  if (first < last) request(first);
+  for (int d = 0; d < Rows::kDepth; ++d) request(first + d, d);
   int group_ends = first;  // the first row of the next group
 #pragma unroll 1
   for (int row = first; row < last; ++row) {
@@ -185,16 +263,21 @@ __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) 
       group_ends = (group + 1) * a.rows_per_group;
     }
     float v[NP][V], x[NP][V];
+    {
+      Piece<T, V> in[2][NP];
+      incoming.take(in);
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+      for (int p = 0; p < NP; ++p)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[p][i] = next_f[p].get(i);
-        x[p][i] = next_x[p].get(i);
-      }
-    if (row + 1 < last) request(row + 1);
+        for (int i = 0; i < V; ++i) {
+          v[p][i] = in[0][p].get(i);
+          x[p][i] = in[1][p].get(i);
+        }
+    }
+    if (!Rows::kSlots) request(row + Rows::kDepth, incoming.freed());
     float mean1, r1, mean2, r2;
     row_statistics<V, NP, LAYER>(a.post_norm, v, live, a.inv_channels, a.epsilon, team_sum, mean1, r1);
+    if (Rows::kSlots) request(row + Rows::kDepth, incoming.freed());  // (what was in the slot has been used)
     const size_t base = (size_t)row * a.channels;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
@@ -207,8 +290,7 @@ __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) 
       }
       if (live[p] && a.sum != nullptr) {
         Piece<T, V> s;
-#pragma unroll
-        for (int i = 0; i < V; ++i) s.set(i, v[p][i]);
+        s.round(v[p]);
         s.store(static_cast<T*>(a.sum) + base + at[p]);
       }
     }
@@ -221,10 +303,11 @@ __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) 
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if constexpr (LAYER)
-            o.set(i, (v[p][i] - mean2) * r2 * pre_gamma[p][i] + pre_beta[p][i]);
+            v[p][i] = (v[p][i] - mean2) * r2 * pre_gamma[p][i] + pre_beta[p][i];
           else
-            o.set(i, v[p][i] * r2 * pre_gamma[p][i]);
+            v[p][i] = v[p][i] * r2 * pre_gamma[p][i];
         }
+        o.round(v[p]);
         o.store(static_cast<T*>(a.out) + base + at[p]);
       }
     if (t == 0 && a.statistics != nullptr) {
@@ -279,7 +362,7 @@ __global__ void __launch_bounds__(1024) residual_norm_long_kernel(const NormArgs
 #pragma unroll
           for (int i = 0; i < V; ++i) total += term(v[i]);
         }
-        return team_sum(total, 0.f).x * a.inv_channels;
+        return team_sum.one(total) * a.inv_channels;
       };
       if (kind == PDNN_NORM_NONE) continue;
       float m = 0.f;
@@ -293,13 +376,15 @@ __global__ void __launch_bounds__(1024) residual_norm_long_kernel(const NormArgs
       float v[V];
       at_sum(c, v);
       Piece<T, V> s, o, pg, pb;
+      float w[V];
       if (a.pre_gamma != nullptr) pg.load(static_cast<const T*>(a.pre_gamma) + c);
       if (a.pre_beta != nullptr) pb.load(static_cast<const T*>(a.pre_beta) + c);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s.set(i, v[i]);
-        o.set(i, (v[i] - mean[1]) * r[1] * (a.pre_gamma != nullptr ? pg.get(i) : 1.f) + (a.pre_beta != nullptr ? pb.get(i) : 0.f));
+        w[i] = (v[i] - mean[1]) * r[1] * (a.pre_gamma != nullptr ? pg.get(i) : 1.f) + (a.pre_beta != nullptr ? pb.get(i) : 0.f);
       }
+      s.round(v);
+      o.round(w);
       if (a.sum != nullptr) s.store(static_cast<T*>(a.sum) + base + c);
       if (a.out != nullptr) o.store(static_cast<T*>(a.out) + base + c);
     }
@@ -320,10 +405,14 @@ __device__ __forceinline__ void unit_rows(const NormArgs& a, long long unit, int
 }
 
 // LAYER: at least one of the norms is a layer norm, or there is a beta: gradients of beta, and sums of u.
+template <typename T, int V, int TEAM, int NP>
+using BackwardRows = Incoming<T, V, NP, 4, 3, block_of(TEAM)>;
 template <typename T, int V, int TEAM, int NP, bool LAYER>
 __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residual_norm_grad_kernel(const NormArgs a) {
   overlap_wait();
+  extern __shared__ __align__(16) char rows_shared[];
   constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM, VL = LAYER ? V : 1;
+  using Rows = BackwardRows<T, V, TEAM, NP>;
   __shared__ float2 slots[2 * (TEAM > 32 ? TEAM / 32 : 1)];
   TeamSum<TEAM> team_sum{slots};
   const int t = (int)threadIdx.x % TEAM;
@@ -346,9 +435,15 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
     for (int i = 0; i < V; ++i) pre_gamma[p][i] = a.pre_gamma == nullptr ? 1.f : live[p] ? g.get(i) : 0.f;
   }
   float d_pre_gamma[NP][V] = {}, d_pre_beta[NP][VL] = {};
-  float* line = a.partial != nullptr ? a.partial + (size_t)team * a.line : nullptr;
-  const T *branch = static_cast<const T*>(a.branch), *sum = static_cast<const T*>(a.residual);
-  const T *sum_grad = static_cast<const T*>(a.sum_grad), *out_grad = static_cast<const T*>(a.out_grad);
+  // the team's line of partial sums; teams of a warp leave theirs to the block, which adds them up
+  float* line = a.partial == nullptr ? nullptr
+                : kTeams > 1         ? reinterpret_cast<float*>(rows_shared + Rows::kSharedBytes) + ((int)threadIdx.x / TEAM) * a.line
+                                     : a.partial + (size_t)team * a.line;
+  if (kTeams > 1 && line != nullptr)
+    for (int c = t; c < (int)a.line; c += TEAM) line[c] = 0.f;
+  Rows incoming(rows_shared);
+  const T* const from[4] = {static_cast<const T*>(a.branch), static_cast<const T*>(a.residual), static_cast<const T*>(a.sum_grad),
+                            static_cast<const T*>(a.out_grad)};
 
 #pragma unroll 1
   for (long long unit = team; unit < units; unit += teams) {
@@ -374,61 +469,53 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
       for (int i = 0; i < V; ++i)
         slope[p][i] = live[p] ? a.scale * (a.gate != nullptr ? activate(a.gate_activation, gate[i]) : 1.f) * gamma[i] : 0.f;
     }
-    Piece<T, V> next_f[NP], next_s[NP], next_ds[NP], next_do[NP];
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {  // (what is never loaded is zero)
-        next_f[p].set(i, 0.f);
-        next_s[p].set(i, 0.f);
-        next_ds[p].set(i, 0.f);
-        next_do[p].set(i, 0.f);
-      }
     float next_stats[4];
-    auto request = [&](int row) {
-      const size_t base = (size_t)row * a.channels;
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        if (live[p]) {
-          next_f[p].load(branch + base + at[p]);
-          next_s[p].load(sum + base + at[p]);
-          if (sum_grad != nullptr) next_ds[p].load(sum_grad + base + at[p]);
-          next_do[p].load(out_grad + base + at[p]);
-        }
+    auto request = [&](int row, int into) { incoming.request(from, (size_t)row * a.channels, row < last, live, at, into); };
+    auto request_statistics = [&](int row) {
+      if (row >= last) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i) next_stats[i] = a.statistics[(size_t)i * a.rows + row];
     };
-    if (first < last) request(first);
+    incoming.slot = 0;  // (every group of the stretch before has been waited for)
+#pragma unroll
+    for (int d = 0; d < Rows::kDepth; ++d) request(first + d, d);
+    request_statistics(first);
 #pragma unroll 1
     for (int row = first; row < last; ++row) {
       const float mean1 = next_stats[0], r1 = next_stats[1], mean2 = next_stats[2], r2 = next_stats[3];
       float u[NP][V], hat[NP][V], f[NP][V], ds[NP][V];
       float a1 = 0.f, a2 = 0.f;
+      {
+        Piece<T, V> in[4][NP];
+        incoming.take(in);
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float g = next_do[p].get(i);
-          hat[p][i] = LAYER ? (live[p] ? (next_s[p].get(i) - mean2) * r2 : 0.f) : next_s[p].get(i) * r2;
-          f[p][i] = LAYER ? (live[p] ? (next_f[p].get(i) - mean1) * r1 : 0.f) : next_f[p].get(i) * r1;
-          ds[p][i] = next_ds[p].get(i);
-          u[p][i] = g * pre_gamma[p][i];
-          d_pre_gamma[p][i] += g * hat[p][i];
-          a1 += u[p][i] * hat[p][i];
-          if constexpr (LAYER) {
-            d_pre_beta[p][i] += g;
-            a2 += u[p][i];
+          for (int i = 0; i < V; ++i) {
+            const float g = in[3][p].get(i);
+            hat[p][i] = LAYER ? (live[p] ? (in[1][p].get(i) - mean2) * r2 : 0.f) : in[1][p].get(i) * r2;
+            f[p][i] = LAYER ? (live[p] ? (in[0][p].get(i) - mean1) * r1 : 0.f) : in[0][p].get(i) * r1;
+            ds[p][i] = in[2][p].get(i);
+            u[p][i] = g * pre_gamma[p][i];
+            d_pre_gamma[p][i] += g * hat[p][i];
+            a1 += u[p][i] * hat[p][i];
+            if constexpr (LAYER) {
+              d_pre_beta[p][i] += g;
+              a2 += u[p][i];
+            }
           }
-        }
-      if (row + 1 < last) request(row + 1);
+      }
+      if (!Rows::kSlots) request(row + Rows::kDepth, incoming.freed());
+      request_statistics(row + 1);
       const size_t base = (size_t)row * a.channels;
       if (a.pre_norm != PDNN_NORM_NONE) {
-        const float2 s = team_sum(a1, a2);
+        const float2 s = team_sum.template sum<LAYER ? 2 : 1>(a1, a2);
         a1 = s.x * a.inv_channels;
         a2 = LAYER && a.pre_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       } else {
         a1 = a2 = 0.f;
       }
+      if (Rows::kSlots) request(row + Rows::kDepth, incoming.freed());  // (what was in the slot has been used)
       float b1 = 0.f, b2 = 0.f;
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
@@ -436,8 +523,7 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
         for (int i = 0; i < V; ++i) ds[p][i] += r2 * (LAYER ? u[p][i] - hat[p][i] * a1 - a2 : u[p][i] - hat[p][i] * a1);
         if (live[p] && a.residual_grad != nullptr) {
           Piece<T, V> o;
-#pragma unroll
-          for (int i = 0; i < V; ++i) o.set(i, ds[p][i]);
+          o.round(ds[p]);
           o.store(static_cast<T*>(a.residual_grad) + base + at[p]);
         }
 #pragma unroll
@@ -452,7 +538,7 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
         }
       }
       if (a.post_norm != PDNN_NORM_NONE) {
-        const float2 s = team_sum(b1, b2);
+        const float2 s = team_sum.template sum<LAYER ? 2 : 1>(b1, b2);
         b1 = s.x * a.inv_channels;
         b2 = LAYER && a.post_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       } else {
@@ -463,7 +549,8 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
         if (live[p] && a.branch_grad != nullptr) {
           Piece<T, V> o;
 #pragma unroll
-          for (int i = 0; i < V; ++i) o.set(i, r1 * (LAYER ? u[p][i] - f[p][i] * b1 - b2 : u[p][i] - f[p][i] * b1));
+          for (int i = 0; i < V; ++i) u[p][i] = r1 * (LAYER ? u[p][i] - f[p][i] * b1 - b2 : u[p][i] - f[p][i] * b1);
+          o.round(u[p]);
           o.store(static_cast<T*>(a.branch_grad) + base + at[p]);
         }
     }
@@ -496,10 +583,12 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
       if (a.parts == 1) {
         Piece<T, V> o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.set(i, d_gate[i] * activation_slope(a.gate_activation, gate[i]));
+        for (int i = 0; i < V; ++i) d_gate[i] *= activation_slope(a.gate_activation, gate[i]);
+        o.round(d_gate);
         o.store(static_cast<T*>(a.gate_grad) + (size_t)group * a.channels + at[p]);
       } else {
-        float* to = a.gate_partial + (size_t)part * a.gate_line + (size_t)group * a.channels + at[p];
+        float* to = a.gate_vector >= 0 ? line + (size_t)a.gate_vector * a.channels + at[p]
+                                       : a.gate_partial + ((size_t)part * groups + group) * a.channels + at[p];
 #pragma unroll
         for (int i = 0; i < V; ++i) to[i] = d_gate[i];
       }
@@ -518,6 +607,16 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
       if constexpr (LAYER) {
         if (a.slot[3] >= 0) line[(size_t)a.slot[3] * a.channels + at[p] + i] = d_pre_beta[p][i];
       }
+    }
+  }
+  if constexpr (kTeams > 1) {
+    __syncthreads();
+    const float* lines = reinterpret_cast<const float*>(rows_shared + Rows::kSharedBytes);
+    for (int c = (int)threadIdx.x; c < (int)a.line; c += kBlock) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTeams; ++w) sum += lines[w * a.line + c];
+      a.partial[(size_t)blockIdx.x * a.line + c] = sum;
     }
   }
 }
@@ -541,7 +640,8 @@ __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const Nor
     int group, part, first, last;
     unit_rows(a, unit, group, part, first, last);
     const T* gate = a.gate != nullptr ? static_cast<const T*>(a.gate) + (size_t)group * a.channels : nullptr;
-    float* gate_line = a.gate_partial != nullptr ? a.gate_partial + (size_t)part * a.gate_line + (size_t)group * a.channels : nullptr;
+    float* gate_line = a.gate_vector >= 0        ? line + (size_t)a.gate_vector * a.channels
+                       : a.gate_partial != nullptr ? a.gate_partial + ((size_t)part * groups + group) * a.channels : nullptr;
     if (gate_line != nullptr)
       for (int c = (int)threadIdx.x; c < a.channels; c += 1024) gate_line[c] = 0.f;
     for (int row = first; row < last; ++row) {
@@ -571,7 +671,7 @@ __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const Nor
           p += g * ((to_f32(sum[base + c]) - st[2]) * st[3]);
           q += g;
         }
-        const float2 s = team_sum(p, q);
+        const float2 s = team_sum.two(p, q);
         a1 = s.x * a.inv_channels;
         a2 = a.pre_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       }
@@ -582,7 +682,7 @@ __global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const Nor
           p += o.u * o.f;
           q += o.u;
         }
-        const float2 s = team_sum(p, q);
+        const float2 s = team_sum.two(p, q);
         b1 = s.x * a.inv_channels;
         b2 = a.post_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       }
@@ -643,8 +743,9 @@ struct Shape {
   static constexpr int team = TEAM, np = NP;
 };
 
-// The smallest team that keeps a row of `pieces` packets (PACKETS) or elements; 0 where none does.
-template <bool PACKETS, typename F>
+// The smallest team that keeps a row of `pieces` packets (PACKETS) or smaller pieces; 0 where none does.  LONG: of packets of
+// four or single elements a thread keeps more.
+template <bool PACKETS, bool LONG, typename F>
 int with_shape(int pieces, F&& f) {
   if constexpr (PACKETS) {
     if (pieces <= 32) return f(Shape<32, 1>{});
@@ -653,20 +754,62 @@ int with_shape(int pieces, F&& f) {
     if (pieces <= 256) return f(Shape<256, 1>{});
     if (pieces <= 512) return f(Shape<512, 1>{});
     if (pieces <= 1024) return f(Shape<512, 2>{});
+    if constexpr (LONG) {
+      if (pieces <= 2048) return f(Shape<1024, 2>{});
+    }
   } else {
     if (pieces <= 128) return f(Shape<32, 4>{});
     if (pieces <= 512) return f(Shape<128, 4>{});
     if (pieces <= 1024) return f(Shape<256, 4>{});
     if (pieces <= 2048) return f(Shape<512, 4>{});
-    if (pieces <= 4096) return f(Shape<512, 8>{});
+    if constexpr (LONG) {
+      if (pieces <= 4096) return f(Shape<512, 8>{});
+    }
   }
   return 0;
 }
 template <typename T, typename F>
-int with_pieces(bool packets, int channels, F&& f) {
+int with_pieces(int width, int channels, F&& f) {
   constexpr int N = Vec16<T>::N;
-  if (packets) return with_shape<true>(channels / N, [&](auto shape) { return f(std::integral_constant<int, N>{}, shape); });
-  return with_shape<false>(channels, [&](auto shape) { return f(std::integral_constant<int, 1>{}, shape); });
+  if (width == N) return with_shape<true, N == 4>(channels / N, [&](auto shape) { return f(std::integral_constant<int, N>{}, shape); });
+  if constexpr (N == 8) {
+    if (width == 2) return with_shape<false, false>(channels / 2, [&](auto shape) { return f(std::integral_constant<int, 2>{}, shape); });
+  }
+  return with_shape<false, true>(channels, [&](auto shape) { return f(std::integral_constant<int, 1>{}, shape); });
+}
+// Elements to a load: a packet, a pair of 16-bit elements or one, by the channels and what all tensors' addresses are multiples of.
+template <typename T>
+int piece_width(int channels, std::initializer_list<const void*> list) {
+  uintptr_t low = 0;
+  for (const void* p : list) low |= reinterpret_cast<uintptr_t>(p);
+  if (channels % Vec16<T>::N == 0 && low % 16 == 0) return Vec16<T>::N;
+  return sizeof(T) == 2 && channels % 2 == 0 && channels <= 4096 && low % 4 == 0 ? 2 : 1;
+}
+
+constexpr int kMostShared = 224 * 1024;
+// As launch_overlapped, with dynamic shared memory, much of it by opting in (once for a kernel and device).
+void launch_rows(void (*kernel)(NormArgs), unsigned grid, unsigned block, int shared, const NormArgs& a, cudaStream_t s) {
+  if (shared > 40 * 1024) {  // (the kernels' own few slots come on top)
+    static std::mutex mu;
+    static std::set<std::pair<int, const void*>> known;
+    const std::pair<int, const void*> key(current_device(), reinterpret_cast<const void*>(kernel));
+    std::lock_guard<std::mutex> lock(mu);
+    if (known.count(key) == 0) {
+      if (cudaFuncSetAttribute(key.second, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return;  // (check_launch reads the error)
+      known.insert(key);
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = (size_t)shared;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;  // (a grid is one wave at most)
+  cudaLaunchKernelEx(&cfg, kernel, a);  // (the caller's check_launch() reads the error)
 }
 
 int check_params(const char* what, int dtype, const PdnnResidualNormParams& p) {
@@ -698,12 +841,6 @@ NormArgs make_args(const PdnnResidualNormParams& p) {
   return a;
 }
 
-bool all_aligned(std::initializer_list<const void*> list) {
-  for (const void* p : list)
-    if (!aligned16(p)) return false;
-  return true;
-}
-
 }  // namespace
 
 int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnResidualNormTensors& t, cudaStream_t s) {
@@ -731,24 +868,22 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
   const bool layer = p.post_norm == PDNN_NORM_LAYER || p.pre_norm == PDNN_NORM_LAYER || t.post_beta != nullptr || t.pre_beta != nullptr;
   return dispatch(dtype, [&](auto type) {
     using T = decltype(type);
-    constexpr int N = Vec16<T>::N;
-    const bool packets = p.channels % N == 0 && all_aligned({t.branch, t.residual, t.post_gamma, t.post_beta, t.gate,
-                                                             t.pre_gamma, t.pre_beta, t.sum, t.output});
-    const int known = with_pieces<T>(packets, p.channels, [&](auto width, auto shape) {
-      constexpr int V = decltype(width)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np, kTeams = block_of(TEAM) / TEAM;
+    const int width = piece_width<T>(p.channels, {t.branch, t.residual, t.post_gamma, t.post_beta, t.gate, t.pre_gamma, t.pre_beta,
+                                                 t.sum, t.output});
+    const int known = with_pieces<T>(width, p.channels, [&](auto elements, auto shape) {
+      constexpr int V = decltype(elements)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np, kTeams = block_of(TEAM) / TEAM;
       // one wave, with a row or more to each team
       const long long wave = (long long)sms * forward_blocks(TEAM, V * NP);
       const unsigned grid = (unsigned)std::min<long long>(wave, ((long long)p.rows + kTeams - 1) / kTeams);
-      if (layer)
-        launch_overlapped(residual_norm_kernel<T, V, TEAM, NP, true>, grid, block_of(TEAM), s, a);
-      else
-        launch_overlapped(residual_norm_kernel<T, V, TEAM, NP, false>, grid, block_of(TEAM), s, a);
+      constexpr int kShared = ForwardRows<T, V, TEAM, NP>::kSharedBytes;
+      launch_rows(layer ? residual_norm_kernel<T, V, TEAM, NP, true> : residual_norm_kernel<T, V, TEAM, NP, false>, grid,
+                  block_of(TEAM), kShared, a, s);
       return 1;
     });
     if (known == 0) {
       const unsigned grid = (unsigned)std::min(p.rows, 2 * sms);
-      if (packets)
-        launch_overlapped(residual_norm_long_kernel<T, N>, grid, 1024, s, a);
+      if (width == Vec16<T>::N)
+        launch_overlapped(residual_norm_long_kernel<T, Vec16<T>::N>, grid, 1024, s, a);
       else
         launch_overlapped(residual_norm_long_kernel<T, 1>, grid, 1024, s, a);
     }
@@ -795,25 +930,20 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
                      g.pre_beta_grad != nullptr || t.post_beta != nullptr;
   return dispatch(dtype, [&](auto type) {
     using T = decltype(type);
-    constexpr int N = Vec16<T>::N;
-    const bool packets = p.channels % N == 0 &&
-                         all_aligned({t.branch, t.sum, t.post_gamma, t.post_beta, t.gate, t.pre_gamma, g.sum_grad, g.output_grad,
-                                      g.branch_grad, g.residual_grad, g.gate_grad});
+    const int width = piece_width<T>(p.channels, {t.branch, t.sum, t.post_gamma, t.post_beta, t.gate, t.pre_gamma, g.sum_grad,
+                                                 g.output_grad, g.branch_grad, g.residual_grad, g.gate_grad});
     const int groups = p.rows / a.rows_per_group;
-    // The cut of the groups for at most `wave` teams, and scratch for what the teams leave: a line to a team of the grid (of
-    // which a block has `to_block`) and one to a group's part.  Returns the blocks, 0 where there is no scratch.
+    // The cut of the groups for at most `wave` teams (of which a block has `to_block`), and scratch for what the blocks leave.
+    // Returns the blocks, 0 where there is no scratch.
     void* scratch = nullptr;
-    long long teams = 0;
-    bool joined = false;  // the gate's sums are a vector of the teams' lines
+    long long blocks = 0;
     auto plan = [&](long long wave, int to_block, bool direct) {
       a.parts = (int)std::max<long long>(1, std::min<long long>(wave / groups, a.rows_per_group));
-      const long long blocks = (std::min<long long>(wave, (long long)groups * a.parts) + to_block - 1) / to_block;
-      teams = blocks * to_block;
+      blocks = (std::min<long long>(wave, (long long)groups * a.parts) + to_block - 1) / to_block;
       const bool gates = g.gate_grad != nullptr && !(direct && a.parts == 1);
-      // (the parts of one group are the teams, but for teams without rows: their vector of the line is then not added)
-      joined = gates && groups == 1 && teams == a.parts;
-      a.line = (size_t)(a.vectors + (joined ? 1 : 0)) * p.channels;
-      const size_t lines = (size_t)teams * a.line, apart = gates && !joined ? (size_t)groups * a.parts * p.channels : 0;
+      a.gate_vector = gates && groups == 1 ? a.vectors : -1;
+      a.line = (size_t)(a.vectors + (a.gate_vector >= 0 ? 1 : 0)) * p.channels;
+      const size_t lines = (size_t)blocks * a.line, apart = gates && groups > 1 ? (size_t)groups * a.parts * p.channels : 0;
       if (lines + apart > 0) {
         if (cudaMallocAsync(&scratch, (lines + apart) * sizeof(float), s) != cudaSuccess) {
           cudaGetLastError();
@@ -821,22 +951,20 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
           return 0u;
         }
         a.partial = lines > 0 ? static_cast<float*>(scratch) : nullptr;
-        if (gates) a.gate_partial = static_cast<float*>(scratch) + (joined ? (size_t)a.vectors * p.channels : lines);
-        a.gate_line = joined ? a.line : (size_t)groups * p.channels;
+        a.gate_partial = apart > 0 ? static_cast<float*>(scratch) + lines : nullptr;
       }
       return (unsigned)blocks;
     };
     unsigned grid = 0;
-    const int known = with_pieces<T>(packets, p.channels, [&](auto width, auto shape) {
-      constexpr int V = decltype(width)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np;
+    const int known = with_pieces<T>(width, p.channels, [&](auto elements, auto shape) {
+      constexpr int V = decltype(elements)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np;
       constexpr int kThreads = block_of(TEAM), kTeams = kThreads / TEAM;
       const long long wave = std::min<long long>((long long)sms * gradient_blocks(TEAM) * kTeams, p.rows);
       grid = plan(wave, kTeams, true);
       if (grid == 0) return 1;
-      if (layer)
-        launch_overlapped(residual_norm_grad_kernel<T, V, TEAM, NP, true>, grid, kThreads, s, a);
-      else
-        launch_overlapped(residual_norm_grad_kernel<T, V, TEAM, NP, false>, grid, kThreads, s, a);
+      const int shared = BackwardRows<T, V, TEAM, NP>::kSharedBytes + (kTeams > 1 ? (int)(kTeams * a.line * sizeof(float)) : 0);
+      launch_rows(layer ? residual_norm_grad_kernel<T, V, TEAM, NP, true> : residual_norm_grad_kernel<T, V, TEAM, NP, false>, grid,
+                  kThreads, shared, a, s);
       return 1;
     });
     if (known == 0) {
@@ -848,16 +976,16 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
     if (status == PDNN_OK && a.partial != nullptr) {
       StoreVectors<T> store;
       store.channels = p.channels;
-      store.gate = joined ? static_cast<const T*>(t.gate) : nullptr;
-      store.gate_vector = joined ? a.vectors : -1;
+      store.gate = static_cast<const T*>(t.gate);
+      store.gate_vector = a.gate_vector;
       store.activation = p.gate_activation;
       for (int i = 0; i < 4; ++i)
         if (a.slot[i] >= 0) store.to[a.slot[i]] = static_cast<T*>(vectors[i]);
-      if (joined) store.to[a.vectors] = static_cast<T*>(g.gate_grad);
-      launch_column_sums(a.partial, (int)teams, a.line, sms, s, store);
+      if (a.gate_vector >= 0) store.to[a.gate_vector] = static_cast<T*>(g.gate_grad);
+      launch_column_sums(a.partial, (int)blocks, a.line, sms, s, store);
       status = check_launch(what);
     }
-    if (status == PDNN_OK && a.gate_partial != nullptr && !joined) {
+    if (status == PDNN_OK && a.gate_partial != nullptr) {
       launch_column_sums(a.gate_partial, a.parts, (size_t)groups * p.channels, sms, s,
                          StoreGate<T>{static_cast<T*>(g.gate_grad), static_cast<const T*>(t.gate), p.gate_activation});
       status = check_launch(what);
