@@ -51,26 +51,6 @@ __device__ __forceinline__ float activation_slope(int act, float z) {
 }
 
 // ---- for results of 16 bits, and with the activation known at compile time --------------------------------
-// Two multiply-adds to an instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)),
-        "l"(*reinterpret_cast<const unsigned long long*>(&c)));
-  return *reinterpret_cast<const float2*>(&r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
-  return *reinterpret_cast<const float2*>(&r);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float exp2_approx(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float reciprocal_approx(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

@@ -581,29 +581,61 @@ __device__ __forceinline__ void store_packet(OutT* p, bool vec, int left, const 
   }
 }
 
-// A CTA's share of the result: it adds up the ranks' partial tiles in their order and finishes what comes of it, a packet to a
-// thread, two packets at a time.
+// The packets of a CTA's share of the result: item i is a packet of line i >> shift.
+struct Share {
+  int rows, rank, m0, n0, swapped, shift, items, cols;
+  __device__ __forceinline__ Share(const FusedArgs& a, int splits, int rank_, int m0_, int n0_, int bn, int packet)
+      : rows(128 / splits), rank(rank_), m0(m0_), n0(n0_), swapped(a.swapped), cols(a.f.cols) {
+    shift = __ffs((swapped ? rows : bn) / packet) - 1;  // (a power of two)
+    items = (swapped ? min(bn, a.f.rows - n0) : min(rows, a.f.rows - m0 - rank * rows)) << shift;
+  }
+  // Row and first column of the result, how many of its columns are inside, and the line and column of the partial tile.
+  __device__ __forceinline__ void place(int i, int packet, long long& r, int& col, int& left, int& line, int& at) const {
+    const int l = i >> shift, c = (i - (l << shift)) * packet;
+    r = swapped ? n0 + l : m0 + rank * rows + l;
+    col = swapped ? m0 + rank * rows + c : n0 + c;
+    left = i < items ? cols - col : 0;
+    line = swapped ? l : rank * rows + l;
+    at = swapped ? rank * rows + c : c;
+  }
+};
+// What is added to a thread's first packet, or its slope taken of, asked for before the ranks meet (whole packets only).
+struct Extras {
+  uint4 bias, aux;
+  bool has_bias, has_aux;
+};
+template <typename OutT>
+__device__ __forceinline__ Extras ask_for_extras(const FusedArgs& a, const Share& share) {
+  constexpr int N = Vec16<OutT>::N;
+  Extras e;
+  e.bias = e.aux = make_uint4(0u, 0u, 0u, 0u);
+  long long r;
+  int col, left, l, c;
+  share.place((int)threadIdx.x, N, r, col, left, l, c);
+  e.has_bias = a.f.bias != nullptr && a.bias_vec && left >= N;
+  e.has_aux = a.f.aux != nullptr && a.aux_vec && left >= N;
+  if (e.has_bias) e.bias = *reinterpret_cast<const uint4*>(static_cast<const OutT*>(a.f.bias) + col);
+  if (e.has_aux) e.aux = *reinterpret_cast<const uint4*>(static_cast<const OutT*>(a.f.aux) + r * a.f.aux_pitch + col);
+  return e;
+}
+
+// Adds up the ranks' partial tiles in their order and finishes what comes of it, a packet to a thread, two packets at a
+// time where few ranks leave registers for it.
 template <typename OutT, int SPLITS>
-__device__ __forceinline__ void finish_share(const FusedArgs& a, uint32_t partial, uint32_t line, int m0, int n0, int bn, int rank) {
-  constexpr int N = Vec16<OutT>::N, rows = 128 / SPLITS;
+__device__ __forceinline__ void finish_share(const FusedArgs& a, const Share& share, uint32_t partial, uint32_t line, const Extras& extras) {
+  constexpr int N = Vec16<OutT>::N, U = SPLITS >= 4 ? 1 : 2;
   const Finish& f = a.f;
-  const int shift = __ffs((a.swapped ? rows : bn) / N) - 1;  // packets in a line of the result, a power of two
-  const int lines = a.swapped ? min(bn, f.rows - n0) : min(rows, f.rows - m0 - rank * rows);
-  const int items = lines << shift;
-  for (int i0 = (int)threadIdx.x; i0 < items; i0 += 2 * kSoloThreads) {
-    float z[2][N];
-    float4 got[2][SPLITS][N / 4];
-    long long r[2];
-    int col[2], left[2];
+  for (int i0 = (int)threadIdx.x; i0 < share.items; i0 += U * kSoloThreads) {
+    float z[U][N];
+    float4 got[U][SPLITS][N / 4];
+    long long r[U];
+    int col[U], left[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i = i0 + u * kSoloThreads, l = i >> shift, c = (i - (l << shift)) * N;
-      r[u] = a.swapped ? n0 + l : m0 + rank * rows + l;
-      col[u] = a.swapped ? m0 + rank * rows + c : n0 + c;
-      left[u] = i < items ? f.cols - col[u] : 0;
+    for (int u = 0; u < U; ++u) {
+      int l, c;
+      share.place(i0 + u * kSoloThreads, N, r[u], col[u], left[u], l, c);
       if (left[u] <= 0) continue;
-      const uint32_t at = partial + (a.swapped ? (uint32_t)l * line + (uint32_t)(rank * rows + c) * 4u
-                                               : (uint32_t)(rank * rows + l) * line + (uint32_t)c * 4u);
+      const uint32_t at = partial + (uint32_t)l * line + (uint32_t)c * 4u;
 #pragma unroll
       for (int k = 0; k < SPLITS; ++k) {
         const uint32_t from = SPLITS == 1 ? at : cluster_map_shared(at, (uint32_t)k);
@@ -612,13 +644,22 @@ __device__ __forceinline__ void finish_share(const FusedArgs& a, uint32_t partia
       }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (left[u] <= 0) continue;
+      const bool first = u == 0 && i0 == (int)threadIdx.x;
       float x[N], b[N];
+      if (first && extras.has_bias)
+        unpack<OutT>(extras.bias, b);
+      else if (f.bias != nullptr)
+        load_packet<OutT>(static_cast<const OutT*>(f.bias) + col[u], a.bias_vec, left[u], b);
+      if (first && extras.has_aux) {
+        unpack<OutT>(extras.aux, x);
+      } else if (f.aux != nullptr) {
+        load_packet<OutT>(static_cast<const OutT*>(f.aux) + r[u] * f.aux_pitch + col[u], a.aux_vec, left[u], x);
+      } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = b[j] = 0.f;
-      if (f.bias != nullptr) load_packet<OutT>(static_cast<const OutT*>(f.bias) + col[u], a.bias_vec, left[u], b);
-      if (f.aux != nullptr) load_packet<OutT>(static_cast<const OutT*>(f.aux) + r[u] * f.aux_pitch + col[u], a.aux_vec, left[u], x);
+        for (int j = 0; j < N; ++j) x[j] = 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < N / 4; ++j) {
         float4 s = got[u][0][j];
@@ -629,8 +670,10 @@ __device__ __forceinline__ void finish_share(const FusedArgs& a, uint32_t partia
         }
         z[u][4 * j] = s.x, z[u][4 * j + 1] = s.y, z[u][4 * j + 2] = s.z, z[u][4 * j + 3] = s.w;
       }
+      if (f.bias != nullptr) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) z[u][j] += b[j];
+        for (int j = 0; j < N; ++j) z[u][j] += b[j];
+      }
       if (f.pre != nullptr) store_packet<OutT>(static_cast<OutT*>(f.pre) + r[u] * f.pre_pitch + col[u], a.pre_vec, left[u], z[u]);
       if (f.gradient) {
         with_activation(f.act, [&](auto act) {
@@ -781,8 +824,10 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   // ------------------------------- partial tile -> shared memory ------------------------------
   // A line of 16 bytes more than it holds: [row][column], or [column][row] where rows are the result's columns.
   const uint32_t line = (uint32_t)(a.swapped ? 128 : bn) * 4u + 16u;
+  grid_dependency_wait();
+  const Share share(a, splits, rank, m0, n0, bn, Vec16<OutT>::N);
+  const Extras extras = ask_for_extras<OutT>(a, share);
   if (warp >= 2) {
-    grid_dependency_wait();
     const int q = warp & 3, row = q * 32 + lane;
     const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
     auto put = [&](int c0, const float* v) {  // 16 columns
@@ -850,12 +895,11 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   cluster_sync_all();
   // ------------------------------- the CTA's share of the result ------------------------------
   if (!*abort_flag) {
-    grid_dependency_wait();
     switch (splits) {
-      case 8: finish_share<OutT, 8>(a, base + 1024u, line, m0, n0, bn, rank); break;
-      case 4: finish_share<OutT, 4>(a, base + 1024u, line, m0, n0, bn, rank); break;
-      case 2: finish_share<OutT, 2>(a, base + 1024u, line, m0, n0, bn, rank); break;
-      default: finish_share<OutT, 1>(a, base + 1024u, line, m0, n0, bn, rank);
+      case 8: finish_share<OutT, 8>(a, share, base + 1024u, line, extras); break;
+      case 4: finish_share<OutT, 4>(a, share, base + 1024u, line, extras); break;
+      case 2: finish_share<OutT, 2>(a, share, base + 1024u, line, extras); break;
+      default: finish_share<OutT, 1>(a, share, base + 1024u, line, extras);
     }
   } else {
     const uint64_t t0 = global_timer_ns();  // copies already issued may still be landing in shared memory

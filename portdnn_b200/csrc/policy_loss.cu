@@ -24,12 +24,6 @@ namespace {
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;  // (log2 e, ln 2)
 
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 struct LossArgs {
   const void *logits, *targets;
   const float *advantages, *old_logp, *ref_logp, *weights;
@@ -45,10 +39,25 @@ struct LossArgs {
 struct alignas(8) Partial {
   float shift, sum;
 };
-__device__ __forceinline__ float scale_to(float from, float to) { return from == to ? 1.f : exp2_fast(from - to); }  // (both may be infinite)
+__device__ __forceinline__ float scale_to(float from, float to) { return from == to ? 1.f : exp2_approx(from - to); }  // (both may be infinite)
 __device__ __forceinline__ Partial merge(Partial a, Partial b) {
   const float shift = fmaxf(a.shift, b.shift);
   return Partial{shift, a.sum * scale_to(a.shift, shift) + b.sum * scale_to(b.shift, shift)};
+}
+
+// The largest entry (NaN passed over).
+__device__ __forceinline__ float packet_max(const Vec16<float>& p) {
+  return fmaxf(fmaxf(p.get(0), p.get(1)), fmaxf(p.get(2), p.get(3)));
+}
+__device__ __forceinline__ float packet_max(const Vec16<__half>& p) {
+  const __half2* h = reinterpret_cast<const __half2*>(&p.raw);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float packet_max(const Vec16<__nv_bfloat16>& p) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&p.raw);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
 }
 
 template <typename T>
@@ -111,31 +120,49 @@ __global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
     return;  // (all CTAs of the cluster alike)
   }
 
-  // (read ahead of every write: the gradient may take the place of the logits)
-  const float chosen = tid == 0 ? to_f32(x[t]) : 0.f;
+  // (read ahead of every write: the gradient may take the place of the logits; and ahead of the row, whose end all wait for)
+  float chosen = 0.f, adv = 0.f, old = 0.f, ref = 0.f;
+  if (tid == 0) {
+    chosen = to_f32(x[t]);
+    adv = a.advantages[row];
+    if (a.old_logp != nullptr) old = a.old_logp[row];
+    if (a.ref_logp != nullptr) ref = a.ref_logp[row];
+  }
   Partial part{-INFINITY, 0.f};
-  auto take = [&](const float* v, int n) {
-    float top = v[0];
-    for (int i = 1; i < n; ++i) top = fmaxf(top, v[i]);
+  // Makes room for a value: false where there is nothing but minus infinity so far (or NaN, which no maximum sees).
+  auto rise = [&](float top) {
     const float shift = top * a.c;
     if (shift > part.shift) {
-      part.sum *= exp2_fast(part.shift - shift);  // (from minus infinity: 0 times 0)
+      part.sum *= exp2_approx(part.shift - shift);  // (from minus infinity: 0 times 0)
       part.shift = shift;
     }
-    if (part.shift == -INFINITY) {  // nothing but minus infinity, or NaN, which fmaxf passes over
-      for (int i = 0; i < n; ++i)
-        if (v[i] != v[i]) part.sum = v[i];
-      return;
-    }
-    float sum = 0.f;
-    for (int i = 0; i < n; ++i) sum += exp2_fast(fmaf(v[i], a.c, -part.shift));
-    part.sum += sum;
+    return part.shift != -INFINITY;
+  };
+  auto take = [&](float v) {
+    if (rise(v))
+      part.sum += exp2_approx(fmaf(v, a.c, -part.shift));
+    else if (v != v)
+      part.sum = v;
   };
   auto take_packet = [&](const Vec16<T>& p) {
-    float v[N];
+    float2 v[N / 2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = to_f32(p.get(i));
-    take(v, N);
+    for (int i = 0; i < N / 2; ++i) v[i] = make_float2(to_f32(p.get(2 * i)), to_f32(p.get(2 * i + 1)));
+    if (rise(packet_max(p))) {
+      float2 sum = both(0.f);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 e = fma2(v[i], both(a.c), both(-part.shift));
+        sum = add2(sum, make_float2(exp2_approx(e.x), exp2_approx(e.y)));
+      }
+      part.sum += sum.x + sum.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (v[i].x != v[i].x) part.sum = v[i].x;
+        if (v[i].y != v[i].y) part.sum = v[i].y;
+      }
+    }
   };
   walk([&](auto whole, int j) {
     Vec16<T> p[kUnroll];
@@ -146,8 +173,7 @@ __global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
     for (int u = 0; u < kUnroll; ++u)
       if (whole || j + u * kStep < tail) take_packet(p[u]);
   }, [&](int j) {
-    const float v = to_f32(x[j]);
-    take(&v, 1);
+    take(to_f32(x[j]));
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -156,8 +182,12 @@ __global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
   }
   if ((tid & 31) == 0) warp_part[tid >> 5] = part;
   __syncthreads();
-  part = warp_part[0];
-  for (int w = 1; w < threads / 32; ++w) part = merge(part, warp_part[w]);
+  // (each warp merges the warps' sums, of which there are a power of two)
+  part = warp_part[(tid & 31) & (threads / 32 - 1)];
+  for (int o = threads / 64; o > 0; o >>= 1) {
+    const Partial other{__shfl_xor_sync(0xFFFFFFFFu, part.shift, o), __shfl_xor_sync(0xFFFFFFFFu, part.sum, o)};
+    part = merge(part, other);
+  }
   if (ranks > 1) {
     if (tid == 0) cta_part = part;
     __syncwarp();
@@ -176,20 +206,19 @@ __global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
     float slope = 0.f, loss = 0.f, lp = 0.f;
     if (!(part.shift == -INFINITY && part.sum == 0.f)) {  // (a row of nothing but minus infinity counts for nothing)
       lp = (fmaf(chosen, a.c, -part.shift) - log2f(part.sum)) * kLn2;
-      const float adv = a.advantages[row];
-      const float ratio = a.old_logp != nullptr ? expf(lp - a.old_logp[row]) : 1.f;
+      const float ratio = a.old_logp != nullptr ? expf(lp - old) : 1.f;
       const float open = ratio * adv, clipped = fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * adv;
       loss = -fminf(open, clipped);
       slope = open <= clipped ? -open : 0.f;
       if (open != open) loss = slope = open;
       if (a.ref_logp != nullptr) {
-        const float d = a.ref_logp[row] - lp, q = expf(d);
+        const float d = ref - lp, q = expf(d);
         loss += a.kl * (q - d - 1.f);
         slope += a.kl * (1.f - q);
       }
       loss *= weight;
       slope *= weight * a.grad_scale * a.inv_temperature;
-      chosen_grad = slope - slope * (exp2_fast(fmaf(chosen, a.c, -part.shift)) / part.sum);
+      chosen_grad = slope - slope * (exp2_approx(fmaf(chosen, a.c, -part.shift)) / part.sum);
     }
     shared_slope = slope;
     if (rank == 0) {
@@ -209,19 +238,22 @@ __global__ void __launch_bounds__(512, 3) policy_loss_kernel(const LossArgs a) {
     if constexpr (sizeof(T) == 2) {
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pair_word<T>(exp2_fast(fmaf(to_f32(p.get(2 * i)), a.c, lift)), exp2_fast(fmaf(to_f32(p.get(2 * i + 1)), a.c, lift))) ^ sign;
+      for (int i = 0; i < 4; ++i) {
+        const float2 e = fma2(make_float2(to_f32(p.get(2 * i)), to_f32(p.get(2 * i + 1))), both(a.c), both(lift));
+        w[i] = pair_word<T>(exp2_approx(e.x), exp2_approx(e.y)) ^ sign;
+      }
       o.raw = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float e = exp2_fast(fmaf(to_f32(p.get(i)), a.c, lift));
+        const float e = exp2_approx(fmaf(to_f32(p.get(i)), a.c, lift));
         o.set(i, from_f32<T>(slope > 0.f ? -e : e));
       }
     }
     return o;
   };
   auto alone = [&](int j) {
-    const float e = exp2_fast(fmaf(to_f32(x[j]), a.c, lift));
+    const float e = exp2_approx(fmaf(to_f32(x[j]), a.c, lift));
     g[j] = from_f32<T>(none ? 0.f : slope > 0.f ? -e : e);
   };
   walk([&](auto whole, int j) {
