@@ -47,6 +47,7 @@ struct alignas(64) FusedArgs {
   int a_mn, b_mn, stages;
   unsigned a_lbo, a_sbo, a_layout, a_kadv, b_lbo, b_sbo, b_layout, b_kadv, idesc;
   int out_tma, aux_tma, pre_tma;
+  int beside;                        // the kernel needs nothing of the one ahead of it: it waits for that one at its end only
   // solo_gemm_kernel
   int bn, splits, blocks_per_split, swapped, tmem_cols;
   int out_vec, aux_vec, pre_vec, bias_vec;  // whole packets at a time
@@ -71,6 +72,10 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t src, i
 // A wait of the whole warp: all lanes learn the same, so that none is left behind at a warp barrier when one gives up.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const FusedArgs& a, unsigned where) {
   return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, a.error_record, a.wait_limit_ns, where));
+}
+
+__device__ __forceinline__ void wait_for_predecessor(const FusedArgs& a) {
+  if (!a.beside) grid_dependency_wait();
 }
 
 // Which parts the i-th product of a step takes, the smallest products first (16-bit operands have one part and one product).
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    grid_dependency_wait();
+    wait_for_predecessor(a);
 #pragma unroll 1
     for (int tile = first; tile < total && ok; tile += step) {
       int m0, n0;
@@ -250,7 +255,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer (rank 0) --------------------------------------
-    grid_dependency_wait();
+    wait_for_predecessor(a);
     grid_launch_dependents();  // the grid is a single wave, and its columns of tensor memory are taken
     if (leader) {
       const uint64_t a_desc0 = make_smem_desc(0, a.a_lbo, a.a_sbo, a.a_layout), b_desc0 = make_smem_desc(0, a.b_lbo, a.b_sbo, a.b_layout);
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     const bool has_aux = f.aux != nullptr, has_pre = f.pre != nullptr;
     // Blocks take the two slots in turn; where the pre-activation is stored, too, it has the second one to itself.
     uint32_t blocks_done = 0, aux_phase = 0u, buf = 0, aph = 0;
-    grid_dependency_wait();
+    wait_for_predecessor(a);
     bool ok = true;
 #pragma unroll 1
     for (int tile = first; tile < total && ok; tile += step) {
@@ -526,6 +531,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
   }
 
   // ------------------------------- teardown ---------------------------------------------------
+  if (a.beside) grid_dependency_wait();  // (who waits for this kernel has waited for both)
   tc_fence_before_sync();
   __syncthreads();
   if (*abort_flag) {  // copies already issued may still be landing in shared memory
@@ -743,7 +749,7 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
 
   if (warp == 0) {
     // ------------------------------- producer ------------------------------------------------
-    grid_dependency_wait();
+    wait_for_predecessor(a);
     grid_launch_dependents();  // (the columns of tensor memory are taken)
     int s = 0;
     uint32_t ph = 0;
@@ -784,7 +790,7 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
     const uint32_t a_kadv = a.a_kadv >> 4, b_kadv = a.b_kadv >> 4, idesc = a.idesc;
     int s = 0;
     uint32_t ph = 0, buf = 0, aph = 0, accumulate = 0u;
-    grid_dependency_wait();
+    wait_for_predecessor(a);
 #pragma unroll 1
     for (int kb = k0; kb < k1; ++kb) {
       const int in_chain = (kb - k0) % kChainSteps;
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
   // ------------------------------- partial tile -> shared memory ------------------------------
   // A line of 16 bytes more than it holds: [row][column], or [column][row] where rows are the result's columns.
   const uint32_t line = (uint32_t)(a.swapped ? 128 : bn) * 4u + 16u;
-  grid_dependency_wait();
+  wait_for_predecessor(a);
   const Share share(a, splits, rank, m0, n0, bn, Vec16<OutT>::N);
   const Extras extras = ask_for_extras<OutT>(a, share);
   if (warp >= 2) {
@@ -906,6 +912,7 @@ __global__ void __launch_bounds__(kSoloThreads, 2) solo_gemm_kernel(const __grid
     while (global_timer_ns() - t0 < 200000ull) {
     }
   }
+  if (a.beside) grid_dependency_wait();
   __syncwarp();
   cluster_sync_all();  // no CTA leaves while another may still read its partial tile
   if (warp == 1) {
@@ -1111,7 +1118,7 @@ int launch_cluster(void (*kernel)(FusedArgs), const FusedArgs& args, unsigned gr
 
 // dtype: of the operands (f16 or bf16); out_dtype: of the finish's tensors.
 template <typename OutT, bool SPLIT>
-int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, int part_k, const Finish& f, cudaStream_t s) {
+int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, int part_k, const Finish& f, bool beside, cudaStream_t s) {
   const int sms = device_sm_count();
   FusedArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -1125,6 +1132,7 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
   a.error_record = tc_error_record_address();
   if (a.error_record == nullptr) return fail(PDNN_ALLOCATION_PROBLEM, "matmul_fused: no error record");
   a.wait_limit_ns = kWaitLimitNs;
+  a.beside = beside;
   a.tiles_m = (x.mn + bm - 1) / bm;
   a.tiles_n = (y.mn + plan.bn - 1) / plan.bn;
   a.group_m = std::min(a.tiles_m, 8);
@@ -1194,13 +1202,13 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
 
 bool fused_gemm_operand_ok(int dtype, const Matrix& m) { return dtype == PDNN_F32 || tma_ok(dtype, m.p, m.pitch, m.rows); }
 
-int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, cudaStream_t s) {
+int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int k, const Finish& f, bool beside, cudaStream_t s) {
   const int sms = device_sm_count();
   Side x{a.p, a.pitch, f.rows, ta}, y{b.p, b.pitch, f.cols, !tb};
   const int kblocks = (k + 63) / 64;
   Plan plan = choose_plan(dtype == PDNN_F32, f.rows, f.cols, x.mn_major != 0, y.mn_major != 0, kblocks, sms);
-  if (dtype == PDNN_F16) return run_plan<__half, false>(plan, dtype, dtype, x, y, k, 0, f, s);
-  if (dtype == PDNN_BF16) return run_plan<__nv_bfloat16, false>(plan, dtype, dtype, x, y, k, 0, f, s);
+  if (dtype == PDNN_F16) return run_plan<__half, false>(plan, dtype, dtype, x, y, k, 0, f, beside, s);
+  if (dtype == PDNN_BF16) return run_plan<__nv_bfloat16, false>(plan, dtype, dtype, x, y, k, 0, f, beside, s);
   // fp32.  Few rows: cutting the weights into parts costs more than multiplying them (4096 x 4096, us, parts / rows: 1 row 59 / 15, 16
   // rows 59 / 47, 32 rows 60 / 78).
   if (!ta && f.rows <= kFewRows) return fused_rows(tb != 0, a, b, k, f, s);
@@ -1243,7 +1251,7 @@ int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int 
   }
   launch_overlapped(split_parts_kernel, split.side[0].blocks + split.side[1].blocks, 256, s, split);
   int st = check_launch("matmul_fused: parts");
-  if (st == PDNN_OK) st = run_plan<float, true>(plan, PDNN_BF16, PDNN_F32, x, y, k, part_k, f, s);
+  if (st == PDNN_OK) st = run_plan<float, true>(plan, PDNN_BF16, PDNN_F32, x, y, k, part_k, f, false, s);
   cudaFreeAsync(scratch, s);
   return st;
 }
