@@ -63,7 +63,7 @@ def _front_command():
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + \
         [f for i in includes for f in ("-isystem", i)] + \
-        [FRONT_SOURCE, "-o", front_path(), "-L" + HERE, "-lportdnn_b200", "-L" + libdir, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+        [FRONT_SOURCE, "-o", front_path(), "-L" + HERE, "-lportdnn_b200", "-L" + libdir, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
          "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 

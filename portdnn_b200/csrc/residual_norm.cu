@@ -272,15 +272,18 @@ __device__ __forceinline__ void row_statistics(int kind, const float (&v)[NP][V]
 }
 
 // Blocks to an SM that the kernels' registers are cut for, by the elements that a thread keeps of a tensor: forward 1024 threads of
-// 64 registers, half as many with more than eight elements; backward 512 threads of 128.
-constexpr int forward_blocks(int team, int elements) { return (elements > 8 ? 512 : 1024) / block_of(team); }
+// 64 registers, half as many with more than eight elements (layer norms: four); backward 512 threads of 128.
+constexpr int forward_blocks(int team, int elements, bool layer) {
+  const int threads = elements > 8 || (layer && elements > 4) ? 512 : 1024;
+  return threads < block_of(team) ? 1 : threads / block_of(team);
+}
 constexpr int gradient_blocks(int team) { return team > 512 ? 1 : 512 / block_of(team); }
 
 // LAYER: at least one of the norms is a layer norm, or there is a beta.
 template <typename T, int V, int TEAM, int NP>
 using ForwardRows = Incoming<T, V, NP, 2, 3, block_of(TEAM)>;
 template <typename T, int V, int TEAM, int NP, bool LAYER>
-__global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP)) residual_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP, LAYER)) residual_norm_kernel(const NormArgs a) {
   overlap_wait();
   extern __shared__ __align__(16) char rows_shared[];
   constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM;
@@ -895,6 +898,7 @@ int with_shape(int pieces, F&& f) {
       if (pieces <= 2048) return f(Shape<1024, 2>{});
     }
   } else {
+    // (eight single elements to a thread: 1999x1003 f32 gradient 22 -> 32 us, half as many loads on their way)
     if (pieces <= 128) return f(Shape<32, 4>{});
     if (pieces <= 512) return f(Shape<128, 4>{});
     if (pieces <= 1024) return f(Shape<256, 4>{});
@@ -1011,7 +1015,7 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
       constexpr bool LAYER = decltype(layered)::value;
       constexpr int V = decltype(elements)::value, TEAM = decltype(shape)::team, NP = decltype(shape)::np, kTeams = block_of(TEAM) / TEAM;
       // one wave, with a row or more to each team
-      const long long wave = (long long)sms * forward_blocks(TEAM, V * NP);
+      const long long wave = (long long)sms * forward_blocks(TEAM, V * NP, LAYER);
       const unsigned grid = (unsigned)std::min<long long>(wave, ((long long)p.rows + kTeams - 1) / kTeams);
       launch_rows(residual_norm_kernel<T, V, TEAM, NP, LAYER>, grid, block_of(TEAM), ForwardRows<T, V, TEAM, NP>::kSharedBytes, a, s);
       return 1;
