@@ -31,6 +31,32 @@ SNNStatus launch(typename Backend::template pointer_type<T const> lhs, typename 
   return SNNStatus{Event{backend.get_queue()}, StatusCode(st)};
 }
 
+/** output = residual + scale * activation(lhs * op(rhs) + bias), one launch; no counterpart in the reference, which issues
+ * a matmul, a binaryop and a pointwise launch.  Sizes and pitches in `params` (its transpose_rhs is set here), tensors of
+ * the epilogue of type T: see PdnnMatmulEpilogue. */
+template <typename T, bool TransposeRHS, typename Backend>
+SNNStatus launch_fused(typename Backend::template pointer_type<T const> lhs, typename Backend::template pointer_type<T const> rhs,
+                       typename Backend::template pointer_type<T> output, PdnnMatmulParams params,
+                       PdnnMatmulEpilogue const& epilogue, Backend& backend, const std::vector<Event>& events = {}) {
+  for (const Event& e : events) e.make_stream_wait(backend.get_queue());
+  params.transpose_rhs = TransposeRHS;
+  const int st = pdnn_matmul_fused(backend::dtype_of<T>::value, lhs, rhs, output, &params, &epilogue, backend.get_queue());
+  return SNNStatus{Event{backend.get_queue()}, StatusCode(st)};
+}
+
+/** The gradients of launch_fused with respect to lhs, rhs and bias: see PdnnMatmulGradient. */
+template <typename T, bool TransposeRHS, typename Backend>
+SNNStatus launch_fused_gradient(typename Backend::template pointer_type<T const> output_grad,
+                                typename Backend::template pointer_type<T const> lhs,
+                                typename Backend::template pointer_type<T const> rhs, PdnnMatmulParams params,
+                                PdnnMatmulGradient const& gradient, Backend& backend, const std::vector<Event>& events = {}) {
+  for (const Event& e : events) e.make_stream_wait(backend.get_queue());
+  params.transpose_rhs = TransposeRHS;
+  const int st = pdnn_matmul_fused_gradient(backend::dtype_of<T>::value, output_grad, lhs, rhs, &params, &gradient,
+                                            backend.get_queue());
+  return SNNStatus{Event{backend.get_queue()}, StatusCode(st)};
+}
+
 }  // namespace matmul
 }  // namespace sycldnn
 #endif

@@ -5,8 +5,8 @@ accumulator to each addition), and fp32 operands, which are multiplied in three 
 bits each, the product of the smaller ones left out).  Activations change by at most 1.2 times what their argument does, and are
 computed to 2^-20 of 1 + |z|.  Each 16-bit rounding adds half a step: of the result, and in gradients of dz, which the tensor
 cores multiply in the tensors' type."""
-import ctypes
 import itertools
+import re
 
 import pytest
 import torch
@@ -14,6 +14,7 @@ import torch
 import portdnn_b200 as pd
 from block_operators import ACTS, DTYPES, act, close, half_step, slope
 from gpu_util import assert_no_device_error
+from launched import launched
 
 pytestmark = pytest.mark.gpu
 
@@ -278,3 +279,46 @@ def test_refusals():
     for f in (lambda: pd.pointwise(pd.ACT_GELU, x), lambda: pd.bias_add(x, b[:16].contiguous(), 16, activation=pd.ACT_SILU)):
         with pytest.raises(pd.PortDNNError):
             f()
+
+
+@pytest.mark.parametrize("m,k,n,dtype,kernel", [
+    (8192, 256, 2048, "bf16", r"pair_gemm_kernelI13__nv_bfloat16Li256ELb0"), (4000, 128, 512, "f16", r"pair_gemm_kernelI6__halfLi128ELb0"),
+    (1, 4096, 4096, "bf16", r"solo_gemm_kernelI13__nv_bfloat16Lb0"), (250, 2048, 1000, "f16", r"solo_gemm_kernelI6__halfLb0"),
+    (4096, 128, 1024, "f32", r"pair_gemm_kernelIfLi128ELb1"), (300, 520, 515, "f32", r"solo_gemm_kernelIfLb1"),
+    (1, 512, 512, "f32", r"rows_product_kernelILi1E"), (16, 512, 511, "f32", r"rows_product_kernelILi8ELi1E")])
+def test_every_kernel_is_reached(m, k, n, dtype, kernel):
+    """The kernels that the other tests' shapes run on, by the names in a captured call."""
+    dt = DTYPES[dtype]
+    x, w = _normal(1, m, k).to(dt), _normal(2, k, n).to(dt)
+    names = [launch.name for launch in launched(lambda: pd.matmul_fused(x, w, activation=pd.ACT_RELU))]
+    assert re.search(kernel, names[-1]), names
+    _forward(m, k, n, False, dtype, "silu", True, True, 1.0, True)
+    _forward(m, k, n, True, dtype, "relu", False, False, 1.0, False)
+
+
+def test_long_sums_in_single_precision():
+    """Where the accumulator's own rounding would show: the error does not grow with the number of terms."""
+    for m, n in ((300, 200), (2300, 1100)):
+        x, w = _normal(1, m, 8192), _normal(2, 8192, n)
+        got, want = pd.matmul_fused(x, w).double(), x.double() @ w.double()
+        # chains of 64 terms in the accumulator (12 additions to a step of two, 24 in all, each off by 2^-23 of the chain's sum at
+        # most), 128 chains added with 2^-24 each: norm-wise, for sums of terms of random signs, 24 2^-23 + sqrt(128) 2^-24
+        assert (got - want).norm() <= (24 * 2.0 ** -23 + 12 * 2.0 ** -24) * want.norm()
+
+
+def test_calls_follow_their_tensors_device_and_stream():
+    """On a stream that waits for the one that makes its inputs; the tensors' device is the current one already on a box of one GPU."""
+    dt = torch.bfloat16
+    x, w = _normal(1, 2000, 2048).to(dt), _normal(2, 2048, 2048, std=0.02).to(dt)
+    want = pd.matmul_fused(pd.matmul_fused(x, w), w)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        y = pd.matmul_fused(x, w)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = pd.matmul_fused(y, w)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+    if torch.cuda.device_count() > 1:
+        there = [t.to("cuda:1") for t in (x, w)]
+        assert torch.equal(pd.matmul_fused(pd.matmul_fused(*there), there[1]).to("cuda:0"), want)
