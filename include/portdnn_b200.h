@@ -322,7 +322,10 @@ int pdnn_matmul(int dtype, int transpose_lhs, int transpose_rhs, const void* lhs
  * other columns are neither read nor written.  No alignment is asked for: operands that the tensor cores cannot read in
  * place (16-bit rows off a 16-byte boundary, or whose pitch is no multiple of 16 bytes) are copied to scratch from the
  * stream-ordered allocator first.  Sums are held in 32 bits; a result is rounded once.  The order in which the products of
- * an output are added depends on the sizes.  Results have the same bits in every call of the same sizes. */
+ * an output are added depends on the sizes.  Results have the same bits in every call of the same sizes, pitches and
+ * alignments.  fp32 operands are multiplied in three bf16 parts with fp32 sums, as exactly as by fp32 multiply-adds; but an
+ * infinite one may make the results that it enters NaN, and values below 2^-110 keep fewer bits.  A result that lies on an
+ * operand, unless said otherwise, is refused where that can be seen. */
 
 /* lhs [m][k], rhs [k][n] (transpose_rhs: [n][k]), output [m][n].  m may be 0. */
 typedef struct PdnnMatmulParams {
@@ -353,8 +356,8 @@ int pdnn_matmul_fused(int dtype, const void* lhs, const void* rhs, void* output,
  *   rhs_grad  = lhs^T * dz, in rhs' own layout
  *   bias_grad = sum of dz over its rows
  * Null results are left out; the residual's gradient is dy itself.  For 16-bit tensors dz is rounded to their type, which is
- * what the tensor cores multiply (bias_grad sums the values ahead of that rounding, unless dz is dy itself).  lhs_grad may
- * not be one of the inputs' buffers.  m == 0 leaves rhs_grad and bias_grad zero. */
+ * what the tensor cores multiply (bias_grad sums the values ahead of that rounding, unless dz is dy itself).  No
+ * result may lie on an input.  m == 0 leaves rhs_grad and bias_grad zero. */
 typedef struct PdnnMatmulGradient {
   int activation; /* PDNN_ACT_NONE: pre_activation is not read */
   float scale;
@@ -382,7 +385,7 @@ typedef struct PdnnResidualNormParams {
   float scale, epsilon;
 } PdnnResidualNormParams;
 
-/* sum or output may be NULL, and residual (zeros).  sum may be the residual's own buffer and output the branch's.
+/* sum or output may be NULL, and residual (zeros).  Either may be the branch's or the residual's own buffer.
  * statistics ([4][rows] floats; may be NULL): mean and reciprocal deviation that post_norm took, and those of pre_norm (0 and 1
  * where a norm takes none); the gradient reads them.  output and statistics are of the sum in 32 bits. */
 typedef struct PdnnResidualNormTensors {
@@ -394,7 +397,8 @@ int pdnn_residual_norm(int dtype, const PdnnResidualNormParams* params, const Pd
 
 /* Its gradients.  Of `tensors` branch, sum, statistics, the gammas, post_beta and the gate are read.  sum_grad is what
  * arrives at the sum by the residual stream (NULL: nothing), output_grad what arrives at the output.  Null results are left
- * out.  residual_grad may be sum_grad's buffer and branch_grad output_grad's.  Sums over rows are taken in a fixed order. */
+ * out.  branch_grad and residual_grad may each be one of the tensors of their size that are read.  Sums over rows are taken in
+ * a fixed order. */
 typedef struct PdnnResidualNormGradients {
   const void *sum_grad, *output_grad;
   void *branch_grad, *residual_grad, *post_gamma_grad, *post_beta_grad, *gate_grad, *pre_gamma_grad, *pre_beta_grad;

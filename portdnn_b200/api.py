@@ -376,7 +376,8 @@ def residual_norm(branch, residual, params, post_gamma=None, post_beta=None, gat
     """The norms around a block with its gate and residual sum (pdnn_residual_norm; no counterpart in the reference):
     sum = residual + scale * gate_activation(gate) * post_norm(branch), out = pre_norm(sum) -> (sum, out, statistics).
     branch, residual (None: zeros), sum and out: dense [rows, channels]; gammas and betas [channels] (None: ones, zeros);
-    gate [gate_groups, channels], a row of it to rows / gate_groups rows.  sum_out may be the residual, out the branch."""
+    gate [gate_groups, channels], a row of it to rows / gate_groups rows.  Either result may be the branch or the
+    residual."""
     return (_F or _front()).residual_norm(branch, residual, params, post_gamma, post_beta, gate, pre_gamma, pre_beta, sum_out,
                                           out)
 
@@ -386,7 +387,8 @@ def residual_norm_grad(sum_grad, output_grad, branch, sum, statistics, params, p
     """Gradients of residual_norm (pdnn_residual_norm_gradient) -> (branch_grad, residual_grad, post_gamma_grad,
     post_beta_grad, gate_grad, pre_gamma_grad, pre_beta_grad), None for parameters that are None.  sum_grad (None: zeros) is
     what arrives at the sum by the residual stream, output_grad what arrives at the normalised output; sum and statistics
-    are the forward call's.  branch_grad may be output_grad, residual_grad sum_grad."""
+    are the forward call's.  branch_grad and residual_grad may each be one of the
+    tensors of their size that are read."""
     return (_F or _front()).residual_norm_grad(sum_grad, output_grad, branch, sum, statistics, params, post_gamma, post_beta,
                                                gate, pre_gamma, pre_beta, branch_grad, residual_grad)
 

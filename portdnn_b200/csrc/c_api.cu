@@ -516,6 +516,17 @@ int pdnn_matmul_fused(int dtype, const void* lhs, const void* rhs, void* output,
   if (st == PDNN_OK) st = fill_pitch(what, e.pre_activation, e.pre_activation_pitch, p.n);
   if (st != PDNN_OK || p.m == 0) return st;
   if (lhs == nullptr || rhs == nullptr || output == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  const long long es = (long long)dtype_size(dtype);
+  auto matrix = [es](const void* q, long long rows, long long cols, long long pitch) { return Extent{q, rows, cols * es, pitch * es}; };
+  const Extent x = matrix(lhs, p.m, p.k, p.lhs_pitch);
+  const Extent w = p.transpose_rhs ? matrix(rhs, p.n, p.k, p.rhs_pitch) : matrix(rhs, p.k, p.n, p.rhs_pitch);
+  const Extent out = matrix(output, p.m, p.n, p.output_pitch), pre = matrix(e.pre_activation, p.m, p.n, e.pre_activation_pitch);
+  const Extent res = matrix(e.residual, p.m, p.n, e.residual_pitch), bias = matrix(e.bias, 1, p.n, p.n);
+  for (const Extent& written : {out, pre})
+    for (const Extent& read : {x, w, bias})
+      if (overlap(written, read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies on an operand", what);
+  if (overlap(out, pre) || overlap(pre, res) || (overlap(out, res) && !same_place(out, res)))
+    return fail(PDNN_INVALID_PARAMETER, "%s: results and residual lie on one another", what);
   return launch_matmul_fused(dtype, lhs, rhs, output, p, e, static_cast<cudaStream_t>(stream));
 }
 
@@ -539,6 +550,19 @@ int pdnn_matmul_fused_gradient(int dtype, const void* output_grad, const void* l
     if ((g.activation != PDNN_ACT_NONE && g.pre_activation == nullptr) ||
         (g.input_activation != PDNN_ACT_NONE && g.lhs_grad != nullptr && g.input_pre_activation == nullptr))
       return fail(PDNN_INVALID_PARAMETER, "%s: an activation's gradient needs what the activation was applied to", what);
+  }
+  const long long es = (long long)dtype_size(dtype);
+  auto matrix = [es](const void* q, long long rows, long long cols, long long pitch) { return Extent{q, rows, cols * es, pitch * es}; };
+  auto weights = [&](const void* q, long long pitch) { return p.transpose_rhs ? matrix(q, p.n, p.k, pitch) : matrix(q, p.k, p.n, pitch); };
+  const Extent results[3] = {matrix(g.lhs_grad, p.m, p.k, g.lhs_grad_pitch), weights(g.rhs_grad, g.rhs_grad_pitch), matrix(g.bias_grad, 1, p.n, p.n)};
+  const Extent inputs[5] = {matrix(output_grad, p.m, p.n, p.output_pitch), matrix(lhs, p.m, p.k, p.lhs_pitch), weights(rhs, p.rhs_pitch),
+                            matrix(g.pre_activation, p.m, p.n, g.pre_activation_pitch),
+                            matrix(g.input_pre_activation, p.m, p.k, g.input_pre_activation_pitch)};
+  for (int i = 0; i < 3; ++i) {
+    for (const Extent& read : inputs)
+      if (overlap(results[i], read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies on an input", what);
+    for (int j = 0; j < i; ++j)
+      if (overlap(results[i], results[j])) return fail(PDNN_INVALID_PARAMETER, "%s: two results lie on one another", what);
   }
   return launch_matmul_fused_gradient(dtype, output_grad, lhs, rhs, p, g, static_cast<cudaStream_t>(stream));
 }

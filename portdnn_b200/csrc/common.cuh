@@ -164,6 +164,24 @@ __device__ __forceinline__ float apply_activation(float v, int act) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// `rows` rows of `row` bytes, `pitch` bytes apart.
+struct Extent {
+  const void* p;
+  long long rows, row, pitch;
+};
+inline bool same_place(const Extent& a, const Extent& b) { return a.p == b.p && a.rows == b.rows && a.row == b.row && (a.rows <= 1 || a.pitch == b.pitch); }
+// Whether two extents share a byte.  (Of rows with different pitches that lie between one another it says so, too.)
+inline bool overlap(Extent a, Extent b) {
+  if (a.rows == 1 && a.row <= b.pitch) a.pitch = b.pitch;
+  if (b.rows == 1 && b.row <= a.pitch) b.pitch = a.pitch;
+  if (a.p == nullptr || b.p == nullptr || a.rows <= 0 || b.rows <= 0) return false;
+  const long long x = (long long)reinterpret_cast<uintptr_t>(a.p), y = (long long)reinterpret_cast<uintptr_t>(b.p);
+  if (x + (a.rows - 1) * a.pitch + a.row <= y || y + (b.rows - 1) * b.pitch + b.row <= x) return false;
+  if (a.pitch != b.pitch) return true;
+  const long long d = ((y - x) % a.pitch + a.pitch) % a.pitch;  // b's rows begin d bytes behind a's
+  return d < a.row || d + b.row > a.pitch;
+}
+
 // Grid for a grid-stride loop over `items`: enough CTAs to fill the device a few times over.
 inline unsigned grid_for(size_t items, int block, int sm_count) {
   size_t need = (items + block - 1) / block;

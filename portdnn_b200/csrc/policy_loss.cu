@@ -332,6 +332,11 @@ int launch_policy_loss(int dtype, const PdnnPolicyLossParams& p, const PdnnPolic
   if (t.loss == nullptr) return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
   if (p.rows > 0 && (t.logits == nullptr || t.targets == nullptr || t.advantages == nullptr || t.token_loss == nullptr || t.logp == nullptr))
     return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  {
+    const long long es = (long long)dtype_size(dtype);
+    const Extent in{t.logits, p.rows, p.vocab * es, p.logits_pitch * es}, out{t.grad, p.rows, p.vocab * es, p.grad_pitch * es};
+    if (overlap(in, out) && !same_place(in, out)) return fail(PDNN_INVALID_PARAMETER, "%s: the gradient lies across the logits", what);
+  }
   const int sms = device_sm_count();
   if (sms <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
   if (p.rows > 0) {

@@ -24,7 +24,6 @@
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
-#include <set>
 #include <type_traits>
 
 namespace pdnn {
@@ -931,13 +930,20 @@ constexpr int kMostShared = 224 * 1024;
 // As launch_overlapped, with dynamic shared memory, much of it by opting in (once for a kernel and device).
 void launch_rows(void (*kernel)(NormArgs), unsigned grid, unsigned block, int shared, const NormArgs& a, cudaStream_t s) {
   if (shared > 40 * 1024) {  // (the kernels' own few slots come on top)
+    struct Entry {
+      void (*kernel)(NormArgs);
+      int device;
+    };
     static std::mutex mu;
-    static std::set<std::pair<int, const void*>> known;
-    const std::pair<int, const void*> key(current_device(), reinterpret_cast<const void*>(kernel));
+    static Entry known[256];
+    static int count = 0;
+    const int device = current_device();
     std::lock_guard<std::mutex> lock(mu);
-    if (known.count(key) == 0) {
-      if (cudaFuncSetAttribute(key.second, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return;  // (check_launch reads the error)
-      known.insert(key);
+    bool found = false;
+    for (int i = 0; i < count; ++i) found = found || (known[i].kernel == kernel && known[i].device == device);
+    if (!found) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return;  // (check_launch reads the error)
+      if (count < 256) known[count++] = Entry{kernel, device};
     }
   }
   cudaLaunchConfig_t cfg = {};
@@ -966,6 +972,14 @@ int check_params(const char* what, int dtype, const PdnnResidualNormParams& p) {
   return PDNN_OK;
 }
 
+Extent whole(int dtype, const PdnnResidualNormParams& p, const void* t) {
+  return Extent{t, p.rows > 0 ? 1 : 0, (long long)p.rows * p.channels * (long long)dtype_size(dtype), (long long)p.rows * p.channels * (long long)dtype_size(dtype)};
+}
+// Whether two tensors of all rows share bytes without being the same one.
+bool partly(int dtype, const PdnnResidualNormParams& p, const void* a, const void* b) {
+  return a != b && overlap(whole(dtype, p, a), whole(dtype, p, b));
+}
+
 NormArgs make_args(const PdnnResidualNormParams& p) {
   NormArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -992,6 +1006,10 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
     return fail(PDNN_INVALID_PARAMETER, "%s: a gate and its groups belong together", what);
   if (p.rows > 0 && (t.branch == nullptr || (t.sum == nullptr && t.output == nullptr)))
     return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
+  for (const void* written : {(const void*)t.sum, (const void*)t.output})
+    for (const void* read : {t.branch, t.residual})
+      if (partly(dtype, p, written, read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies across an input", what);
+  if (overlap(whole(dtype, p, t.sum), whole(dtype, p, t.output))) return fail(PDNN_INVALID_PARAMETER, "%s: the results lie on one another", what);
   const int sms = device_sm_count();
   if (sms <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
   if (p.rows == 0) return PDNN_OK;
@@ -1044,6 +1062,11 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
   if (p.rows > 0 && (t.branch == nullptr || t.sum == nullptr || t.statistics == nullptr || g.output_grad == nullptr))
     return fail(PDNN_INVALID_PARAMETER, "%s: null tensor", what);
   if (g.gate_grad != nullptr && p.gate_groups == 0) return fail(PDNN_INVALID_PARAMETER, "%s: there is no gate", what);
+  for (const void* written : {(const void*)g.branch_grad, (const void*)g.residual_grad})
+    for (const void* read : {t.branch, (const void*)t.sum, g.sum_grad, g.output_grad})
+      if (partly(dtype, p, written, read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies across an input", what);
+  if (overlap(whole(dtype, p, g.branch_grad), whole(dtype, p, g.residual_grad)))
+    return fail(PDNN_INVALID_PARAMETER, "%s: the results lie on one another", what);
   const int sms = device_sm_count();
   if (sms <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
   NormArgs a = make_args(p);

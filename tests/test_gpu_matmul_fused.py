@@ -322,3 +322,26 @@ def test_calls_follow_their_tensors_device_and_stream():
     if torch.cuda.device_count() > 1:
         there = [t.to("cuda:1") for t in (x, w)]
         assert torch.equal(pd.matmul_fused(pd.matmul_fused(*there), there[1]).to("cuda:0"), want)
+
+
+def test_results_on_operands_are_refused_and_slices_beside_them_are_not():
+    dt = torch.bfloat16
+    wide = _normal(1, 300, 512).to(dt)
+    w, r = _normal(2, 128, 128).to(dt), _normal(3, 300, 128).to(dt)
+    x = wide[:, :128]
+    want = pd.matmul_fused(x, w, residual=r)
+    got = pd.matmul_fused(x, w, residual=r, out=wide[:, 256:384])  # beside the operand, in the same rows
+    assert torch.equal(got, want)
+    pre = torch.empty_like(want)
+    for bad in (dict(out=x), dict(out=wide[:, 64:192]),
+                dict(out=pre, pre_activation=pre), dict(pre_activation=r), dict(pre_activation=x)):
+        with pytest.raises((pd.PortDNNError, ValueError)):
+            pd.matmul_fused(x, w, residual=r, **bad)
+    # the residual shifted by a row is not the residual in place
+    tall = torch.cat([r, r[:1]])
+    with pytest.raises(pd.PortDNNError):
+        pd.matmul_fused(x, w, residual=tall[:-1], out=tall[1:])
+    dy = _normal(4, 300, 128).to(dt)
+    for bad in (dict(lhs_grad=dy), dict(rhs_grad=w), dict(lhs_grad=x), dict(bias_grad=w[5])):
+        with pytest.raises(pd.PortDNNError):
+            pd.matmul_fused_grad(dy, x.contiguous() if "lhs_grad" not in bad else x, w, **bad)

@@ -199,6 +199,9 @@ def test_refusals():
                 dict(grad=torch.empty((6, 101), device="cuda"))):
         with pytest.raises(ValueError):
             pd.policy_loss(**{**s, **bad})
+    wide = torch.zeros((6, 150), device="cuda")
+    with pytest.raises(pd.PortDNNError):  # the gradient across the logits
+        pd.policy_loss(**{**s, "logits": wide[:, :100]}, grad=wide[:, 50:])
     for bad in (dict(temperature=0.0), dict(temperature=float("nan")), dict(clip_low=-0.1), dict(clip_high=float("nan"))):
         with pytest.raises(pd.PortDNNError):
             pd.policy_loss(**s, **bad)

@@ -272,3 +272,27 @@ def test_refusals():
         pd.residual_norm_grad(x, x, x, x, torch.ones(31, device="cuda"), params(8, 64))
     with pytest.raises(TypeError):
         pd.residual_norm(x, x, pd.pool_params(1, 4, 4, 1, 2, 2))
+
+
+def test_results_across_inputs_are_refused():
+    x = torch.ones((9, 64), device="cuda")
+    p = pd.residual_norm_params(8, 64)
+    a, b = x[:8], x[1:]
+    for bad in (dict(sum_out=b), dict(out=b), dict(sum_out=a, out=a)):
+        with pytest.raises(pd.PortDNNError):
+            pd.residual_norm(a, a.clone(), p, **bad)
+    total, out, statistics = pd.residual_norm(a.clone(), a.clone(), p)
+    for bad in (dict(branch_grad=b), dict(residual_grad=b), dict(branch_grad=total, residual_grad=total)):
+        with pytest.raises(pd.PortDNNError):
+            pd.residual_norm_grad(a, a, a, total, statistics, p, **bad)
+
+
+def test_results_in_any_input_s_place():
+    for channels in (72, 1003, 4096, 40000):
+        s, p, vectors, got, grads = _both(30, channels, "rms", "layer", 1, "none", 1.0, "bf16")
+        b, r = s["branch"].clone(), s["residual"].clone()
+        total, out, _ = pd.residual_norm(b, r, p, sum_out=b, out=r, **vectors)
+        assert torch.equal(total, got[0]) and torch.equal(out, got[1])
+        b, total = s["branch"].clone(), got[0].clone()
+        again = pd.residual_norm_grad(s["sum_grad"], s["out_grad"], b, total, got[2], p, branch_grad=total, residual_grad=b, **vectors)
+        assert all(u is v or torch.equal(u, v) for u, v in zip(grads, again))
