@@ -377,7 +377,7 @@ int pdnn_matmul_fused_gradient(int dtype, const void* output_grad, const void* l
  * post_norm normalises what the block has put out, pre_norm what the next block reads.  A norm takes each row's mean
  * square (PDNN_NORM_RMS), or mean and variance (PDNN_NORM_LAYER), over its channels.  Tensors are dense [rows][channels];
  * gammas and betas have `channels` entries (NULL: ones and zeros); the gate is [gate_groups][channels], and each of its rows
- * serves rows / gate_groups consecutive rows (1: all rows; rows: each row its own).  rows may be 0. */
+ * serves rows / gate_groups consecutive rows (1: all rows; rows: each row its own).  rows may be 0; neither count passes 0x7FFF0000. */
 typedef enum PdnnNorm { PDNN_NORM_NONE = 0, PDNN_NORM_RMS = 1, PDNN_NORM_LAYER = 2 } PdnnNorm;
 typedef struct PdnnResidualNormParams {
   int rows, channels, post_norm, pre_norm;
@@ -416,7 +416,7 @@ int pdnn_residual_norm_gradient(int dtype, const PdnnResidualNormParams* params,
  * weights (NULL: ones): floats, one to a row.  loss: one float, the sum of token_loss; token_loss, logp: [rows] floats.
  * grad (NULL: forward only) has the logits' type and may be their own buffer, with the same pitch.
  * A row counts for nothing - loss, logp and gradient 0, whatever its logits hold - where its weight is 0 or its target
- * lies outside [0, vocab); so does one whose logits are all minus infinity.  rows may be 0. */
+ * lies outside [0, vocab); so does one whose logits are all minus infinity.  rows may be 0; neither count passes 0x7FFF0000. */
 typedef struct PdnnPolicyLossParams {
   int rows, vocab, target_bytes;
   float clip_low, clip_high, kl, temperature, grad_scale;

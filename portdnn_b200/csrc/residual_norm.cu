@@ -197,7 +197,7 @@ struct NormArgs {
   void *branch_grad, *residual_grad, *gate_grad;
   // Partial sums: a line of `line` floats to a block, the parameter vectors' behind one another, the gate's too (vector
   // gate_vector) where there is one group; with more groups (gate_vector -1) the gate's are [parts][groups][channels].
-  float *partial, *gate_partial;
+  float *partial, *gate_partial, *row_sums;
   size_t line;
   int parts;    // stretches of rows that a group is cut into
   int vectors;  // parameter vectors with a gradient
@@ -403,46 +403,84 @@ __global__ void __launch_bounds__(block_of(TEAM), forward_blocks(TEAM, V * NP, L
   }
 }
 
-// Rows that no team can keep: a block walks the row once for each sum and once more for the results.
+// What a thread that keeps no row does with V of its columns.
 template <typename T, int V>
-__global__ void __launch_bounds__(1024) residual_norm_long_kernel(const NormArgs a) {
+struct LongRow {
+  const NormArgs& a;
+  static __device__ __forceinline__ void load(const T* p, size_t at, float missing, float (&to)[V]) {
+    Piece<T, V> v;
+    if (p != nullptr) v.load(p + at);
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[i] = p != nullptr ? v.get(i) : missing;
+  }
+  // scale * act(gate) of a group's columns
+  __device__ __forceinline__ void gate(int group, int c, float (&raw)[V], float (&factor)[V]) const {
+    load(a.gate != nullptr ? static_cast<const T*>(a.gate) + (size_t)group * a.channels : nullptr, c, 0.f, raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) factor[i] = a.scale;
+    if (a.gate != nullptr)
+      with_activation(a.gate_activation, [&](auto act) {  // (one way through the switch for all)
+#pragma unroll
+        for (int i = 0; i < V; ++i) factor[i] *= activate(decltype(act)::value, raw[i]);
+      });
+  }
+  // the result's gradient g, u and hat of the norm before the next block
+  __device__ __forceinline__ void before(size_t at, float mean, float r, const float (&gamma)[V], float (&g)[V], float (&u)[V], float (&hat)[V]) const {
+    load(static_cast<const T*>(a.out_grad), at, 0.f, g);
+    load(static_cast<const T*>(a.residual), at, 0.f, hat);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      u[i] = g[i] * gamma[i];
+      hat[i] = (hat[i] - mean) * r;
+    }
+  }
+  // the sum's gradient and hat of the norm behind the block
+  __device__ __forceinline__ void behind(size_t at, float mean, float r, float r2, float a1, float a2, const float (&u)[V], const float (&hat)[V],
+                                         float (&ds)[V], float (&f)[V]) const {
+    load(static_cast<const T*>(a.sum_grad), at, 0.f, ds);
+    load(static_cast<const T*>(a.branch), at, 0.f, f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      ds[i] += r2 * (u[i] - hat[i] * a1 - a2);
+      f[i] = (f[i] - mean) * r;
+    }
+  }
+};
+
+constexpr int kLongThreads = 512;
+constexpr int long_blocks(int v) { return v == 1 ? 4 : 3; }
+// Rows that no team can keep: a block walks the row once for each sum and once more for the results (1000x20000 bf16 83 us, 1.9 TB/s:
+// bound by the latency of its walks).
+template <typename T, int V>
+__global__ void __launch_bounds__(kLongThreads, long_blocks(V)) residual_norm_long_kernel(const NormArgs a) {
   overlap_wait();
-  __shared__ float2 slots[64];
-  TeamSum<1024> team_sum{slots};
+  __shared__ float2 slots[2 * kLongThreads / 32];
+  TeamSum<kLongThreads> team_sum{slots};
+  const LongRow<T, V> long_row{a};
   const T *branch = static_cast<const T*>(a.branch), *residual = static_cast<const T*>(a.residual);
   for (int row = (int)blockIdx.x; row < a.rows; row += (int)gridDim.x) {
     const size_t base = (size_t)row * a.channels;
-    const T* gate = a.gate != nullptr ? static_cast<const T*>(a.gate) + (size_t)(row / a.rows_per_group) * a.channels : nullptr;
     float mean[2] = {0.f, 0.f}, r[2] = {1.f, 1.f};
     auto at_sum = [&](int c, float (&v)[V]) {  // V entries of the sum, in 32 bits
-      Piece<T, V> f, x, g, pg, pb;
-      f.load(branch + base + c);
-      if (residual != nullptr) x.load(residual + base + c);
-      if (gate != nullptr) g.load(gate + c);
-      if (a.post_gamma != nullptr) pg.load(static_cast<const T*>(a.post_gamma) + c);
-      if (a.post_beta != nullptr) pb.load(static_cast<const T*>(a.post_beta) + c);
+      float f[V], k[V], gamma[V], beta[V];
+      long_row.load(branch, base + c, 0.f, f);
+      long_row.load(residual, base + c, 0.f, v);
+      long_row.gate(row / a.rows_per_group, c, gamma, k);
+      long_row.load(static_cast<const T*>(a.post_gamma), c, 1.f, gamma);
+      long_row.load(static_cast<const T*>(a.post_beta), c, 0.f, beta);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float n = (f.get(i) - mean[0]) * r[0] * (a.post_gamma != nullptr ? pg.get(i) : 1.f) +
-                        (a.post_beta != nullptr ? pb.get(i) : 0.f);
-        const float k = gate != nullptr ? a.scale * activate(a.gate_activation, g.get(i)) : a.scale;
-        v[i] = (residual != nullptr ? x.get(i) : 0.f) + k * n;
-      }
+      for (int i = 0; i < V; ++i) v[i] += k[i] * ((f[i] - mean[0]) * r[0] * gamma[i] + beta[i]);
     };
     for (int which = 0; which < 2; ++which) {
       const int kind = which == 0 ? a.post_norm : a.pre_norm;
       auto sum_of = [&](auto&& term) {
         float total = 0.f;
-        for (int c = (int)threadIdx.x * V; c < a.channels; c += 1024 * V) {
+        for (int c = (int)threadIdx.x * V; c < a.channels; c += kLongThreads * V) {
           float v[V];
-          if (which == 0) {
-            Piece<T, V> f;
-            f.load(branch + base + c);
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = f.get(i);
-          } else {
+          if (which == 0)
+            long_row.load(branch, base + c, 0.f, v);
+          else
             at_sum(c, v);
-          }
 #pragma unroll
           for (int i = 0; i < V; ++i) total += term(v[i]);
         }
@@ -456,17 +494,15 @@ __global__ void __launch_bounds__(1024) residual_norm_long_kernel(const NormArgs
       r[which] = q;
     }
     __syncthreads();  // (the results may take the place of the inputs)
-    for (int c = (int)threadIdx.x * V; c < a.channels; c += 1024 * V) {
+    for (int c = (int)threadIdx.x * V; c < a.channels; c += kLongThreads * V) {
       float v[V];
       at_sum(c, v);
-      Piece<T, V> s, o, pg, pb;
-      float w[V];
-      if (a.pre_gamma != nullptr) pg.load(static_cast<const T*>(a.pre_gamma) + c);
-      if (a.pre_beta != nullptr) pb.load(static_cast<const T*>(a.pre_beta) + c);
+      Piece<T, V> s, o;
+      float w[V], gamma[V], beta[V];
+      long_row.load(static_cast<const T*>(a.pre_gamma), c, 1.f, gamma);
+      long_row.load(static_cast<const T*>(a.pre_beta), c, 0.f, beta);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        w[i] = (v[i] - mean[1]) * r[1] * (a.pre_gamma != nullptr ? pg.get(i) : 1.f) + (a.pre_beta != nullptr ? pb.get(i) : 0.f);
-      }
+      for (int i = 0; i < V; ++i) w[i] = (v[i] - mean[1]) * r[1] * gamma[i] + beta[i];
       s.round(v);
       o.round(w);
       if (a.sum != nullptr) s.store(static_cast<T*>(a.sum) + base + c);
@@ -489,6 +525,8 @@ __device__ __forceinline__ void unit_rows(const NormArgs& a, long long unit, int
 }
 
 // LAYER: at least one of the norms is a layer norm, or there is a beta: gradients of beta, and sums of u.
+// (One row at a time: with two, whose reductions lie side by side, the registers for them are missing - 8192x2048 bf16 48.7 -> 51.3
+// us, 16384x1024 48 -> 70.  Bound by issue slots and the two reductions a row: 8192x2048 bf16, eight gates, 48 us, 4.2 TB/s.)
 template <typename T, int V, int TEAM, int NP>
 using BackwardRows = Incoming<T, V, NP, 4, 3, block_of(TEAM)>;
 template <typename T, int V, int TEAM, int NP, bool LAYER>
@@ -523,8 +561,10 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
   float* line = a.partial == nullptr ? nullptr
                 : kTeams > 1         ? reinterpret_cast<float*>(rows_shared + Rows::kSharedBytes) + ((int)threadIdx.x / TEAM) * a.line
                                      : a.partial + (size_t)team * a.line;
-  if (kTeams > 1 && line != nullptr)
+  if (kTeams > 1 && line != nullptr) {
     for (int c = t; c < (int)a.line; c += TEAM) line[c] = 0.f;
+    __syncthreads();  // (other threads write what a stretch leaves)
+  }
   Rows incoming(rows_shared);
   const T* const from[4] = {static_cast<const T*>(a.branch), static_cast<const T*>(a.residual), static_cast<const T*>(a.sum_grad),
                             static_cast<const T*>(a.out_grad)};
@@ -721,85 +761,120 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
   }
 }
 
-// Rows that no team can keep: a block walks its row three times, and the partial sums over rows are lines in memory that
-// the block adds to (nobody else touches them).
-template <typename T>
-__global__ void __launch_bounds__(1024) residual_norm_grad_long_kernel(const NormArgs a) {
+// Rows that no team can keep, in two launches: a block to a row for the four sums over it (row_sums, [4][rows]), then a thread to V
+// columns, which walks down a stretch of rows with the parameters and their sums in registers.  Two reads of everything, the second
+// one from L2 in part (us, a block to a row for it all, its sums over rows in memory / so: 1000x20000
+// bf16 468 / 135, 1000x16384 f32 249 / 155, 1000x20001 bf16, by element, 549 / 373).
+template <typename T, int V>
+__global__ void __launch_bounds__(kLongThreads, 2) residual_norm_grad_rows_kernel(const NormArgs a) {
   overlap_wait();
-  __shared__ float2 slots[64];
-  TeamSum<1024> team_sum{slots};
-  const int groups = a.rows / a.rows_per_group;
-  const long long units = (long long)groups * a.parts;
-  const T *branch = static_cast<const T*>(a.branch), *sum = static_cast<const T*>(a.residual);
-  const T *sum_grad = static_cast<const T*>(a.sum_grad), *out_grad = static_cast<const T*>(a.out_grad);
-  float* line = a.partial != nullptr ? a.partial + (size_t)blockIdx.x * a.line : nullptr;
-  if (line != nullptr)
-    for (int c = (int)threadIdx.x; c < a.channels; c += 1024)
-      for (size_t k = c; k < a.line; k += a.channels) line[k] = 0.f;
-  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    int group, part, first, last;
-    unit_rows(a, unit, group, part, first, last);
-    const T* gate = a.gate != nullptr ? static_cast<const T*>(a.gate) + (size_t)group * a.channels : nullptr;
-    float* gate_line = a.gate_vector >= 0        ? line + (size_t)a.gate_vector * a.channels
-                       : a.gate_partial != nullptr ? a.gate_partial + ((size_t)part * groups + group) * a.channels : nullptr;
-    if (gate_line != nullptr)
-      for (int c = (int)threadIdx.x; c < a.channels; c += 1024) gate_line[c] = 0.f;
-    for (int row = first; row < last; ++row) {
-      const size_t base = (size_t)row * a.channels;
-      float st[4];
-      for (int i = 0; i < 4; ++i) st[i] = a.statistics[(size_t)i * a.rows + row];
-      float a1 = 0.f, a2 = 0.f, b1 = 0.f, b2 = 0.f;
-      // one element's way: gradient of the sum, of the normalised branch, and what the parameters receive
-      struct Step { float ds, u, f, n, dn, g, hat; };
-      auto step = [&](int c) {
-        Step o;
-        o.g = to_f32(out_grad[base + c]);
-        o.hat = (to_f32(sum[base + c]) - st[2]) * st[3];
-        const float u = o.g * (a.pre_gamma != nullptr ? to_f32(static_cast<const T*>(a.pre_gamma)[c]) : 1.f);
-        o.ds = (sum_grad != nullptr ? to_f32(sum_grad[base + c]) : 0.f) + st[3] * (u - o.hat * a1 - a2);
-        o.f = (to_f32(branch[base + c]) - st[0]) * st[1];
-        const float gamma = a.post_gamma != nullptr ? to_f32(static_cast<const T*>(a.post_gamma)[c]) : 1.f;
-        o.n = o.f * gamma + (a.post_beta != nullptr ? to_f32(static_cast<const T*>(a.post_beta)[c]) : 0.f);
-        o.dn = o.ds * a.scale * (gate != nullptr ? activate(a.gate_activation, to_f32(gate[c])) : 1.f);
-        o.u = o.dn * gamma;
-        return o;
-      };
-      if (a.pre_norm != PDNN_NORM_NONE) {
-        float p = 0.f, q = 0.f;
-        for (int c = (int)threadIdx.x; c < a.channels; c += 1024) {
-          const float g = to_f32(out_grad[base + c]) * (a.pre_gamma != nullptr ? to_f32(static_cast<const T*>(a.pre_gamma)[c]) : 1.f);
-          p += g * ((to_f32(sum[base + c]) - st[2]) * st[3]);
-          q += g;
+  __shared__ float2 slots[2 * kLongThreads / 32];
+  TeamSum<kLongThreads> team_sum{slots};
+  const LongRow<T, V> long_row{a};
+  for (int row = (int)blockIdx.x; row < a.rows; row += (int)gridDim.x) {
+    const size_t base = (size_t)row * a.channels;
+    float st[4];
+    for (int i = 0; i < 4; ++i) st[i] = a.statistics[(size_t)i * a.rows + row];
+    float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    for (int which = 0; which < 2; ++which) {
+      const int kind = which == 0 ? a.pre_norm : a.post_norm;
+      if (kind == PDNN_NORM_NONE) continue;
+      float p = 0.f, q = 0.f;
+      for (int c = (int)threadIdx.x * V; c < a.channels; c += kLongThreads * V) {
+        float gamma[V], g[V], u[V], hat[V], f[V];
+        long_row.load(static_cast<const T*>(a.pre_gamma), c, 1.f, gamma);
+        long_row.before(base + c, st[2], st[3], gamma, g, u, hat);
+        if (which == 0) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) p += u[i] * hat[i], q += u[i];
+        } else {
+          long_row.behind(base + c, st[0], st[1], st[3], s[0].x, s[0].y, u, hat, g, f);
+          float raw[V];
+          long_row.gate(row / a.rows_per_group, c, raw, hat);
+          long_row.load(static_cast<const T*>(a.post_gamma), c, 1.f, gamma);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float v = g[i] * hat[i] * gamma[i];
+            p += v * f[i];
+            q += v;
+          }
         }
-        const float2 s = team_sum.two(p, q);
-        a1 = s.x * a.inv_channels;
-        a2 = a.pre_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       }
-      if (a.post_norm != PDNN_NORM_NONE) {
-        float p = 0.f, q = 0.f;
-        for (int c = (int)threadIdx.x; c < a.channels; c += 1024) {
-          const Step o = step(c);
-          p += o.u * o.f;
-          q += o.u;
-        }
-        const float2 s = team_sum.two(p, q);
-        b1 = s.x * a.inv_channels;
-        b2 = a.post_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
-      }
-      __syncthreads();  // (the results may take the place of the inputs)
-      for (int c = (int)threadIdx.x; c < a.channels; c += 1024) {
-        const Step o = step(c);
-        if (a.residual_grad != nullptr) static_cast<T*>(a.residual_grad)[base + c] = from_f32<T>(o.ds);
-        if (a.branch_grad != nullptr) static_cast<T*>(a.branch_grad)[base + c] = from_f32<T>(st[1] * (o.u - o.f * b1 - b2));
-        if (line != nullptr) {
-          const float add[4] = {o.dn * o.f, o.dn, o.g * o.hat, o.g};
-          for (int k = 0; k < 4; ++k)
-            if (a.slot[k] >= 0) line[(size_t)a.slot[k] * a.channels + c] += add[k];
-        }
-        if (gate_line != nullptr) gate_line[c] += o.ds * a.scale * o.n;
-      }
+      s[which] = team_sum.two(p, q);
+      s[which].x *= a.inv_channels;
+      s[which].y = kind == PDNN_NORM_LAYER ? s[which].y * a.inv_channels : 0.f;
+    }
+    if (threadIdx.x == 0) {
+      a.row_sums[row] = s[0].x;
+      a.row_sums[(size_t)a.rows + row] = s[0].y;
+      a.row_sums[2 * (size_t)a.rows + row] = s[1].x;
+      a.row_sums[3 * (size_t)a.rows + row] = s[1].y;
     }
   }
+}
+
+constexpr int kColumnThreads = 128;
+template <typename T, int V>
+__global__ void __launch_bounds__(kColumnThreads, 4) residual_norm_grad_columns_kernel(const NormArgs a) {
+  overlap_wait();
+  const int c = ((int)blockIdx.x * kColumnThreads + (int)threadIdx.x) * V, groups = a.rows / a.rows_per_group;
+  if (c >= a.channels) return;
+  const LongRow<T, V> long_row{a};
+  float pre_gamma[V], gamma[V], sums[4][V] = {};  // (of the gradients of post gamma, post beta, pre gamma, pre beta)
+  long_row.load(static_cast<const T*>(a.pre_gamma), c, 1.f, pre_gamma);
+  long_row.load(static_cast<const T*>(a.post_gamma), c, 1.f, gamma);
+  float* line = a.partial != nullptr ? a.partial + (size_t)blockIdx.y * a.line + c : nullptr;
+  for (long long unit = blockIdx.y; unit < (long long)groups * a.parts; unit += gridDim.y) {
+    int group, part, first, last;
+    unit_rows(a, unit, group, part, first, last);
+    float raw[V], factor[V], p_sum[V] = {}, q_sum[V] = {};
+    long_row.gate(group, c, raw, factor);
+#pragma unroll 2
+    for (int row = first; row < last; ++row) {
+      float st[4], by[4], g[V], u[V], hat[V], ds[V], f[V];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        st[i] = a.statistics[(size_t)i * a.rows + row];
+        by[i] = a.row_sums[(size_t)i * a.rows + row];
+      }
+      const size_t at = (size_t)row * a.channels + c;
+      long_row.before(at, st[2], st[3], pre_gamma, g, u, hat);
+      long_row.behind(at, st[0], st[1], st[3], by[0], by[1], u, hat, ds, f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        sums[2][i] += g[i] * hat[i];
+        sums[3][i] += g[i];
+        p_sum[i] += ds[i] * f[i];
+        q_sum[i] += ds[i];
+        u[i] = st[1] * (ds[i] * factor[i] * gamma[i] - f[i] * by[2] - by[3]);
+      }
+      Piece<T, V> o;
+      if (a.residual_grad != nullptr) {
+        o.round(ds);
+        o.store(static_cast<T*>(a.residual_grad) + at);
+      }
+      if (a.branch_grad != nullptr) {
+        o.round(u);
+        o.store(static_cast<T*>(a.branch_grad) + at);
+      }
+    }
+    float beta[V];
+    long_row.load(static_cast<const T*>(a.post_beta), c, 0.f, beta);
+    float* gate_line = a.gate_vector >= 0        ? line + (size_t)a.gate_vector * a.channels
+                       : a.gate_partial != nullptr ? a.gate_partial + ((size_t)part * groups + group) * a.channels + c : nullptr;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      sums[0][i] += factor[i] * p_sum[i];
+      sums[1][i] += factor[i] * q_sum[i];
+      if (gate_line != nullptr) gate_line[i] = a.scale * (gamma[i] * p_sum[i] + beta[i] * q_sum[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (a.slot[k] >= 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) line[(size_t)a.slot[k] * a.channels + i] = sums[k][i];
+    }
 }
 
 // ---- the second stage: the blocks' lines, and the gate's parts, added up in a fixed order, both in one launch --------------
@@ -962,6 +1037,8 @@ void launch_rows(void (*kernel)(NormArgs), unsigned grid, unsigned block, int sh
 int check_params(const char* what, int dtype, const PdnnResidualNormParams& p) {
   if (dtype < PDNN_F32 || dtype > PDNN_BF16) return fail(PDNN_INVALID_PARAMETER, "%s: unknown dtype %d", what, dtype);
   if (p.rows < 0 || p.channels <= 0) return fail(PDNN_INVALID_PARAMETER, "%s: %d rows of %d channels", what, p.rows, p.channels);
+  if (p.rows > 0x7FFF0000 || p.channels > 0x7FFF0000)  // (kernels count a little past them)
+    return fail(PDNN_INVALID_PARAMETER, "%s: %d rows of %d channels are too many", what, p.rows, p.channels);
   for (int kind : {p.post_norm, p.pre_norm})
     if (kind < PDNN_NORM_NONE || kind > PDNN_NORM_LAYER) return fail(PDNN_INVALID_PARAMETER, "%s: unknown norm %d", what, kind);
   if (p.gate_groups < 0 || (p.gate_groups > 0 && p.rows % p.gate_groups != 0))
@@ -1042,11 +1119,11 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
         layer ? with_pieces<T, true>(width, p.channels, [&](auto elements, auto shape) { return run(std::true_type{}, elements, shape); })
               : with_pieces<T, false>(width, p.channels, [&](auto elements, auto shape) { return run(std::false_type{}, elements, shape); });
     if (known == 0) {
-      const unsigned grid = (unsigned)std::min(p.rows, 2 * sms);
+      const unsigned grid = (unsigned)std::min(p.rows, long_blocks(width) * sms);
       if (width == Vec16<T>::N)
-        launch_overlapped(residual_norm_long_kernel<T, Vec16<T>::N>, grid, 1024, s, a);
+        launch_overlapped(residual_norm_long_kernel<T, Vec16<T>::N>, grid, kLongThreads, s, a);
       else
-        launch_overlapped(residual_norm_long_kernel<T, 1>, grid, 1024, s, a);
+        launch_overlapped(residual_norm_long_kernel<T, 1>, grid, kLongThreads, s, a);
     }
     return check_launch(what);
   });
@@ -1102,6 +1179,7 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
     // The cut of the groups for at most `wave` teams (of which a block has `to_block`), and scratch for what the blocks leave.
     // Returns the blocks, 0 where there is no scratch.
     void* scratch = nullptr;
+    size_t more = 0;  // floats for the rows' sums
     long long blocks = 0;
     auto plan = [&](long long wave, int to_block, bool direct) {
       a.parts = (int)std::max<long long>(1, std::min<long long>(wave / groups, a.rows_per_group));
@@ -1110,14 +1188,15 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
       a.gate_vector = gates && groups == 1 ? a.vectors : -1;
       a.line = (size_t)(a.vectors + (a.gate_vector >= 0 ? 1 : 0)) * p.channels;
       const size_t lines = (size_t)blocks * a.line, apart = gates && groups > 1 ? (size_t)groups * a.parts * p.channels : 0;
-      if (lines + apart > 0) {
-        if (cudaMallocAsync(&scratch, (lines + apart) * sizeof(float), s) != cudaSuccess) {
+      if (lines + apart + more > 0) {
+        if (cudaMallocAsync(&scratch, (lines + apart + more) * sizeof(float), s) != cudaSuccess) {
           cudaGetLastError();
           scratch = nullptr;
           return 0u;
         }
         a.partial = lines > 0 ? static_cast<float*>(scratch) : nullptr;
         a.gate_partial = apart > 0 ? static_cast<float*>(scratch) + lines : nullptr;
+        a.row_sums = static_cast<float*>(scratch) + lines + apart;
       }
       return (unsigned)blocks;
     };
@@ -1134,8 +1213,20 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
       return 1;
     });
     if (known == 0) {
-      grid = plan(std::min<long long>(p.rows, 2ll * sms), 1, false);
-      if (grid > 0) launch_overlapped(residual_norm_grad_long_kernel<T>, grid, 1024, s, a);
+      auto run = [&](auto elements) {
+        constexpr int V = decltype(elements)::value;
+        const int tiles = (p.channels + kColumnThreads * V - 1) / (kColumnThreads * V);
+        // (a wave of blocks; a grid's second dimension ends at 65535)
+        more = 4 * (size_t)p.rows;
+        grid = plan(std::min<long long>(p.rows, std::max(1, 4 * sms / tiles)), 1, false);
+        if (grid == 0) return;
+        launch_overlapped(residual_norm_grad_rows_kernel<T, V>, (unsigned)std::min(p.rows, 4 * sms), kLongThreads, s, a);
+        launch_overlapped(residual_norm_grad_columns_kernel<T, V>, dim3((unsigned)tiles, grid), kColumnThreads, s, a);
+      };
+      if (width == Vec16<T>::N)
+        run(std::integral_constant<int, Vec16<T>::N>{});
+      else
+        run(std::integral_constant<int, 1>{});
     }
     if (grid == 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: cannot allocate scratch", what);
     int status = check_launch(what);

@@ -56,6 +56,12 @@ def test_residual_norm_parameters():
     assert pd.lib().pdnn_residual_norm(0, None, None, None) == INVALID
 
 
+@pytest.mark.parametrize("sizes", [dict(rows=2 ** 31 - 1, channels=1), dict(rows=1, channels=2 ** 31 - 1)])
+def test_residual_norm_counts_past_its_sizes(sizes):
+    assert _norm(**sizes) == INVALID
+    assert b"too many" in pd.lib().pdnn_last_error()
+
+
 def test_policy_loss_parameters():
     def run(rows=4, vocab=100, target_bytes=8, low=0.2, high=0.2, temperature=1.0, pitch=100, grad_pitch=100, dtype=0):
         p = PolicyLossParams(rows, vocab, target_bytes, low, high, 0.1, temperature, 1.0, pitch, grad_pitch)

@@ -147,6 +147,14 @@ def test_rows(rows, channels):
     _both(rows, channels, "layer", "rms", 0, "none", 1.0, "f16", residual=False)
 
 
+# rows that no team keeps: more rows than blocks, groups cut into stretches, more groups than blocks walk at once
+@pytest.mark.parametrize("post,pre", [("rms", "rms"), ("layer", "rms"), ("none", "layer"), ("none", "none")])
+@pytest.mark.parametrize("rows,channels,groups,dtype", [(700, 8200, 0, "bf16"), (700, 8200, 7, "f16"), (320, 9001, 1, "bf16"),
+                                                        (400, 8200, 400, "bf16"), (200, 8196, 2, "f32")])
+def test_long_rows(rows, channels, groups, dtype, post, pre):
+    _both(rows, channels, post, pre, groups, "sigmoid" if groups else "none", 0.7, dtype)
+
+
 @pytest.mark.parametrize("activation", sorted(ACTS))
 def test_gate_activations(activation):
     _both(64, 128, "rms", "rms", 4, activation, 1.0, "f32")
