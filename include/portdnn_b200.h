@@ -327,7 +327,7 @@ int pdnn_matmul(int dtype, int transpose_lhs, int transpose_rhs, const void* lhs
  * infinite one may make the results that it enters NaN, and values below 2^-110 keep fewer bits.  A result that lies on an
  * operand, unless said otherwise, is refused where that can be seen. */
 
-/* lhs [m][k], rhs [k][n] (transpose_rhs: [n][k]), output [m][n].  m may be 0. */
+/* lhs [m][k], rhs [k][n] (transpose_rhs: [n][k]), output [m][n].  m may be 0; none of the three passes 0x7FFF0000. */
 typedef struct PdnnMatmulParams {
   int m, k, n, transpose_rhs;
   long long lhs_pitch, rhs_pitch, output_pitch;
@@ -387,7 +387,8 @@ typedef struct PdnnResidualNormParams {
 
 /* sum or output may be NULL, and residual (zeros).  Either may be the branch's or the residual's own buffer.
  * statistics ([4][rows] floats; may be NULL): mean and reciprocal deviation that post_norm took, and those of pre_norm (0 and 1
- * where a norm takes none); the gradient reads them.  output and statistics are of the sum in 32 bits. */
+ * where a norm takes none); the gradient reads them.  output and statistics are of the sum in 32 bits.  Results on the
+ * vectors, or across a tensor, are refused. */
 typedef struct PdnnResidualNormTensors {
   const void *branch, *residual, *post_gamma, *post_beta, *gate, *pre_gamma, *pre_beta;
   void *sum, *output;
@@ -416,7 +417,7 @@ int pdnn_residual_norm_gradient(int dtype, const PdnnResidualNormParams* params,
  * weights (NULL: ones): floats, one to a row.  loss: one float, the sum of token_loss; token_loss, logp: [rows] floats.
  * grad (NULL: forward only) has the logits' type and may be their own buffer, with the same pitch.
  * A row counts for nothing - loss, logp and gradient 0, whatever its logits hold - where its weight is 0 or its target
- * lies outside [0, vocab); so does one whose logits are all minus infinity.  rows may be 0; neither count passes 0x7FFF0000. */
+ * lies outside [0, vocab); so does one whose logits are all minus infinity.  rows may be 0. */
 typedef struct PdnnPolicyLossParams {
   int rows, vocab, target_bytes;
   float clip_low, clip_high, kl, temperature, grad_scale;

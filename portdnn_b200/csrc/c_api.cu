@@ -5,6 +5,7 @@
 #include "simt_gemm.cuh"
 #include "tc_gemm.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 namespace pdnn {
@@ -482,6 +483,8 @@ namespace {
 int check_matmul_fused(const char* what, int dtype, PdnnMatmulParams& p) {
   if (dtype < PDNN_F32 || dtype > PDNN_BF16) return fail(PDNN_INVALID_PARAMETER, "%s: unknown dtype %d", what, dtype);
   if (p.m < 0 || p.k <= 0 || p.n <= 0) return fail(PDNN_INVALID_PARAMETER, "%s: sizes %d, %d, %d", what, p.m, p.k, p.n);
+  if (std::max(std::max(p.m, p.k), p.n) > 0x7FFF0000)  // (tiles count a little past them)
+    return fail(PDNN_INVALID_PARAMETER, "%s: sizes %d, %d, %d are too large", what, p.m, p.k, p.n);
   p.transpose_rhs = p.transpose_rhs != 0;
   struct {
     long long* pitch;

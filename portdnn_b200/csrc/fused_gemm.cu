@@ -28,7 +28,8 @@ namespace {
 using namespace umma;
 
 // Reduction elements of a stage: a 128-byte row of 16-bit elements; of an fp32 operand's parts, three times as many bytes, half
-// of that (two stages of 72 KB leave a pair waiting for its copies: 1.9 us to 64 elements, four of 36 KB: kept busy).
+// of that, for stages enough ahead (1024x1024x1024, 64 / 32 elements: 26.5 / 25.0 us; pairs are as fast either way, bound by their
+// products, of which one of 256x128x16 is issued every 107 cycles).
 constexpr int step_k(bool split) { return split ? 32 : 64; }
 constexpr int kChainSteps = 2;     // fp32: stages whose products the accumulator takes before it is emptied
 constexpr int kMostStages = 12;
@@ -1214,6 +1215,7 @@ int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int 
   if (!ta && f.rows <= kFewRows) return fused_rows(tb != 0, a, b, k, f, s);
   // parts behind one another along K
   const int part_k = kblocks * 64;
+  if (3ll * part_k > 0x7FFF0000ll) return fail(PDNN_INDEX_EXCEEDED, "matmul_fused: an fp32 sum of %d products is too long", k);  // (TMA counts in 32 bits)
   const Matrix* from[2] = {&a, &b};
   Side* side[2] = {&x, &y};
   size_t bytes[2], cols[2];

@@ -1057,6 +1057,15 @@ bool partly(int dtype, const PdnnResidualNormParams& p, const void* a, const voi
   return a != b && overlap(whole(dtype, p, a), whole(dtype, p, b));
 }
 
+// Whether a result of all rows lies on a vector that other rows still read.
+bool on_vectors(int dtype, const PdnnResidualNormParams& p, const PdnnResidualNormTensors& t, const void* written) {
+  const long long row = (long long)p.channels * (long long)dtype_size(dtype);
+  const Extent result = whole(dtype, p, written);
+  for (const void* v : {t.post_gamma, t.post_beta, t.pre_gamma, t.pre_beta})
+    if (overlap(result, Extent{v, 1, row, row})) return true;
+  return overlap(result, Extent{t.gate, 1, row * p.gate_groups, row * p.gate_groups});
+}
+
 NormArgs make_args(const PdnnResidualNormParams& p) {
   NormArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -1086,6 +1095,7 @@ int launch_residual_norm(int dtype, const PdnnResidualNormParams& p, const PdnnR
   for (const void* written : {(const void*)t.sum, (const void*)t.output})
     for (const void* read : {t.branch, t.residual})
       if (partly(dtype, p, written, read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies across an input", what);
+  if (on_vectors(dtype, p, t, t.sum) || on_vectors(dtype, p, t, t.output)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies on a vector", what);
   if (overlap(whole(dtype, p, t.sum), whole(dtype, p, t.output))) return fail(PDNN_INVALID_PARAMETER, "%s: the results lie on one another", what);
   const int sms = device_sm_count();
   if (sms <= 0) return fail(PDNN_ALLOCATION_PROBLEM, "%s: no sm_100 CUDA device", what);
@@ -1142,6 +1152,8 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
   for (const void* written : {(const void*)g.branch_grad, (const void*)g.residual_grad})
     for (const void* read : {t.branch, (const void*)t.sum, g.sum_grad, g.output_grad})
       if (partly(dtype, p, written, read)) return fail(PDNN_INVALID_PARAMETER, "%s: a result lies across an input", what);
+  if (on_vectors(dtype, p, t, g.branch_grad) || on_vectors(dtype, p, t, g.residual_grad))
+    return fail(PDNN_INVALID_PARAMETER, "%s: a result lies on a vector", what);
   if (overlap(whole(dtype, p, g.branch_grad), whole(dtype, p, g.residual_grad)))
     return fail(PDNN_INVALID_PARAMETER, "%s: the results lie on one another", what);
   const int sms = device_sm_count();

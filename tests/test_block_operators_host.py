@@ -41,6 +41,12 @@ def test_matmul_fused_parameters():
         assert pd.lib().pdnn_last_error()
 
 
+@pytest.mark.parametrize("sizes", [(2 ** 31 - 1, 1, 1), (1, 2 ** 31 - 1, 1), (1, 1, 2 ** 31 - 1)])
+def test_matmul_fused_counts_past_its_sizes(sizes):
+    assert _fused(params=sizes + (0, 0, 0, 0)) == INVALID
+    assert b"too large" in pd.lib().pdnn_last_error()
+
+
 def _norm(rows=8, channels=64, post=1, pre=1, groups=0, act=-1, epsilon=1e-6, dtype=0):
     p = pd.ResidualNormParams(rows, channels, post, pre, groups, act, 1.0, epsilon)
     tensors, gradients = (ctypes.c_void_p * 10)(), (ctypes.c_void_p * 9)()
@@ -60,6 +66,21 @@ def test_residual_norm_parameters():
 def test_residual_norm_counts_past_its_sizes(sizes):
     assert _norm(**sizes) == INVALID
     assert b"too many" in pd.lib().pdnn_last_error()
+
+
+def test_norm_results_on_vectors():
+    p = pd.ResidualNormParams(8, 64, 1, 1, 0, -1, 1.0, 1e-6)
+    far = [0x10000000 * (i + 1) for i in range(10)]  # (addresses that nothing reads: branch, residual, five vectors, sum, output, statistics)
+    far[4] = None
+    for result in (7, 8):
+        for vector in (2, 3, 5, 6):
+            at = list(far)
+            at[result] = far[vector] - 8 * 64 * 4 + 16
+            assert pd.lib().pdnn_residual_norm(0, ctypes.byref(p), (ctypes.c_void_p * 10)(*at), None) == INVALID
+            assert b"vector" in pd.lib().pdnn_last_error()
+            gradients = (ctypes.c_void_p * 9)(0xB0000000, 0xC0000000, *((at[result], None) if result == 7 else (None, at[result])))
+            assert pd.lib().pdnn_residual_norm_gradient(0, ctypes.byref(p), (ctypes.c_void_p * 10)(*far), gradients, None) == INVALID
+            assert b"vector" in pd.lib().pdnn_last_error()
 
 
 def test_policy_loss_parameters():
