@@ -1035,7 +1035,7 @@ struct Plan {
 
 // Estimated times of the plans in us, from what they measured over 24 shapes of 1 to 8192 rows (a step is 64 elements of K).
 // A pair's step takes 0.34 us at 256 columns and 0.23 at 128 (an SM pulls its 24 KB of operands through L2 no faster), two
-// thirds of that with few clusters in flight, behind 5.5 and 4.7 us of launch, ramp and end.  A CTA alone takes 0.2 to 0.29 us a step
+// thirds of that with few clusters in flight (but for fp32, whose products bound it: 2000x777x300 28.7 us, single CTAs 23.1), behind 5.5 and 4.7 us of launch, ramp and end.  A CTA alone takes 0.2 to 0.29 us a step
 // by its columns, half as much again where two share an SM, behind 3 us, 0.017 a column for its end and 0.45 for each
 // partial tile that it adds.
 Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_major, int kblocks, int sms) {
@@ -1047,7 +1047,7 @@ Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_majo
     if (split && bn == 256) continue;
     const long long all = tiles(m, 256) * tiles(n, bn);
     const double waves = (double)tiles(all, sms / 2), busy = std::min(1.0, (double)all / (sms / 2));
-    const double step = (bn == 256 ? 0.34 : 0.23) * (0.6 + 0.4 * busy);
+    const double step = (bn == 256 ? 0.34 : 0.23) * (split ? 1.0 : 0.6 + 0.4 * busy);
     const double t = waves * kblocks * step * products + (bn == 256 ? 5.5 : 4.7) + (split ? 2.0 : 0.0);
     if (t < least) least = t, best = Plan{true, bn, 1, false};
   }

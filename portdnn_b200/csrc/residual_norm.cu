@@ -211,7 +211,7 @@ struct NormArgs {
 // its eight elements.)
 template <int TEAM>
 struct TeamSum {
-  float2* slots;  // the team's, [2][TEAM / 32]
+  float2* slots;  // the team's, [2][TEAM / 32]; twice as many for three values
   int turn = 0;
   template <int COUNT>
   __device__ __forceinline__ float2 sum(float a, float b) {
@@ -243,6 +243,34 @@ struct TeamSum {
       }
     }
     return make_float2(a, b);
+  }
+  // Three values at once (one barrier, and twelve shuffles where one after another takes 27): two steps leave a lane with one of them.
+  __device__ __forceinline__ float3 three(float a, float b, float c) {
+    const int lane = (int)threadIdx.x & 31;
+    const bool odd = (lane & 1) != 0, upper = (lane & 2) != 0;
+    float x = odd ? b : a, y = odd ? 0.f : c;
+    x += __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 1);
+    y += __shfl_xor_sync(0xFFFFFFFFu, odd ? c : 0.f, 1);
+    float v = upper ? y : x;  // lanes 0 to 3 of a group of four: a, b, c, nothing
+    v += __shfl_xor_sync(0xFFFFFFFFu, upper ? x : y, 2);
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if constexpr (TEAM > 32) {
+      constexpr int W = TEAM / 32;
+      float* mine = reinterpret_cast<float*>(slots) + turn * (4 * W);
+      turn ^= 1;
+      if (lane < 4) mine[((int)(threadIdx.x >> 5) & (W - 1)) * 4 + lane] = v;
+      if (TEAM >= 256)
+        __syncthreads();
+      else  // (a block has several teams)
+        umma::named_barrier_sync(1 + threadIdx.x / TEAM, TEAM);
+      v = mine[lane & (4 * W - 1)];
+#pragma unroll
+      for (int w = 32; w < 4 * W; w += 32) v += mine[w + lane];
+#pragma unroll
+      for (int o = 4; o < (W < 8 ? 4 * W : 32); o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    }
+    return make_float3(__shfl_sync(0xFFFFFFFFu, v, 0), __shfl_sync(0xFFFFFFFFu, v, 1), __shfl_sync(0xFFFFFFFFu, v, 2));
   }
   __device__ __forceinline__ float one(float a) { return sum<1>(a, 0.f).x; }
   __device__ __forceinline__ float2 two(float a, float b) { return sum<2>(a, b); }
@@ -526,7 +554,9 @@ __device__ __forceinline__ void unit_rows(const NormArgs& a, long long unit, int
 
 // LAYER: at least one of the norms is a layer norm, or there is a beta: gradients of beta, and sums of u.
 // (One row at a time: with two, whose reductions lie side by side, the registers for them are missing - 8192x2048 bf16 48.7 -> 51.3
-// us, 16384x1024 48 -> 70.  Bound by issue slots and the two reductions a row: 8192x2048 bf16, eight gates, 48 us, 4.2 TB/s.)
+// us, 16384x1024 48 -> 70.  Bound by issue slots
+// and a row's reductions: 16384x4096 bf16 5.9 TB/s, 8192x2048 with eight gates 48 us, 4.2 TB/s.  One reduction of three sums for two of one:
+// 16384x4096 145.9 -> 137.6 us, 16384x1024 48.1 -> 45.5, 20000x512 34.5 -> 32.6, but 20000x100 19.5 -> 20.9.)
 template <typename T, int V, int TEAM, int NP>
 using BackwardRows = Incoming<T, V, NP, 4, 3, block_of(TEAM)>;
 template <typename T, int V, int TEAM, int NP, bool LAYER>
@@ -535,8 +565,8 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
   extern __shared__ __align__(16) char rows_shared[];
   constexpr int kBlock = block_of(TEAM), kTeams = kBlock / TEAM, VL = LAYER ? V : 1;
   using Rows = BackwardRows<T, V, TEAM, NP>;
-  __shared__ float2 slots[2 * kBlock / 32];
-  TeamSum<TEAM> team_sum{slots + (int)threadIdx.x / TEAM * (2 * TEAM / 32)};
+  __shared__ float2 slots[4 * kBlock / 32];
+  TeamSum<TEAM> team_sum{slots + (int)threadIdx.x / TEAM * (4 * TEAM / 32)};
   const int t = (int)threadIdx.x % TEAM;
   const long long team = (long long)blockIdx.x * kTeams + (int)threadIdx.x / TEAM, teams = (long long)gridDim.x * kTeams;
   const int groups = a.rows / a.rows_per_group;
@@ -637,29 +667,50 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
         a1 = dot<V, NP>(u, hat);
         if constexpr (LAYER) a2 = total<V, NP>(u);
       }
+      float b1 = 0.f, b2 = 0.f;
+      if constexpr (!LAYER) {
+        // ds = ds0 - hat * r2 * a1 with ds0 = sum_grad + r2 * u, so b1 = mean(slope f ds) is mean(slope f ds0) - r2 * a1 * mean(slope
+        // f hat): the row's three sums are taken at once.  (No more cancels than in ds itself.)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          float k[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) k[i] = r2;
+          fma_all<V>(ds[p], u[p], k, ds[p]);
+          mul_all<V>(u[p], slope[p], f[p]);
+        }
+        b1 = dot<V, NP>(u, ds);
+        b2 = dot<V, NP>(u, hat);
+      }
       if (!Rows::kSlots) request(row + Rows::kDepth, incoming.freed());
       request_statistics(row + 1);
       const size_t base = (size_t)row * a.channels;
-      if (a.pre_norm != PDNN_NORM_NONE) {
-        const float2 s = team_sum.template sum<LAYER ? 2 : 1>(a1, a2);
+      if constexpr (LAYER) {
+        const float2 s = a.pre_norm != PDNN_NORM_NONE ? team_sum.two(a1, a2) : make_float2(0.f, 0.f);
         a1 = s.x * a.inv_channels;
-        a2 = LAYER && a.pre_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
+        a2 = a.pre_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       } else {
-        a1 = a2 = 0.f;
+        float3 s = make_float3(0.f, 0.f, 0.f);
+        if (a.pre_norm != PDNN_NORM_NONE || a.post_norm != PDNN_NORM_NONE) s = team_sum.three(a1, b1, b2);
+        a1 = a.pre_norm != PDNN_NORM_NONE ? -r2 * (s.x * a.inv_channels) : 0.f;
+        b1 = a.post_norm != PDNN_NORM_NONE ? fmaf(a1, s.z, s.y) * a.inv_channels : 0.f;
       }
       if (Rows::kSlots) request(row + Rows::kDepth, incoming.freed());  // (what was in the slot has been used)
-      float b1 = 0.f, b2 = 0.f;
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         float k1[V], k2[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          k1[i] = -a1;
+          k1[i] = LAYER ? -a1 : a1;
           k2[i] = r2;
           if constexpr (LAYER) u[p][i] -= a2;
         }
-        fma_all<V>(u[p], hat[p], k1, u[p]);
-        fma_all<V>(ds[p], u[p], k2, ds[p]);
+        if constexpr (LAYER) {
+          fma_all<V>(u[p], hat[p], k1, u[p]);
+          fma_all<V>(ds[p], u[p], k2, ds[p]);
+        } else {
+          fma_all<V>(ds[p], hat[p], k1, ds[p]);
+        }
         if (live[p] && a.residual_grad != nullptr) {
           Piece<T, V> o;
           o.round(ds[p]);
@@ -672,14 +723,11 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
           for (int i = 0; i < V; ++i) q_sum[p][i] += ds[p][i];
         }
       }
-      b1 = dot<V, NP>(u, f);
-      if constexpr (LAYER) b2 = total<V, NP>(u);
-      if (a.post_norm != PDNN_NORM_NONE) {
-        const float2 s = team_sum.template sum<LAYER ? 2 : 1>(b1, b2);
+      if constexpr (LAYER) {
+        float2 s = make_float2(0.f, 0.f);
+        if (a.post_norm != PDNN_NORM_NONE) s = team_sum.two(dot<V, NP>(u, f), total<V, NP>(u));
         b1 = s.x * a.inv_channels;
-        b2 = LAYER && a.post_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
-      } else {
-        b1 = b2 = 0.f;
+        b2 = a.post_norm == PDNN_NORM_LAYER ? s.y * a.inv_channels : 0.f;
       }
 #pragma unroll
       for (int p = 0; p < NP; ++p)
@@ -689,7 +737,8 @@ __global__ void __launch_bounds__(block_of(TEAM), gradient_blocks(TEAM)) residua
 #pragma unroll
           for (int i = 0; i < V; ++i) k[i] = -b1;
           fma_all<V>(u[p], f[p], k, u[p]);
-          add_mul<V>(u[p], u[p], LAYER ? -b2 : 0.f, r1);
+          if constexpr (LAYER) add_mul<V>(u[p], u[p], -b2, r1);
+          else mul_by<V>(u[p], u[p], r1);
           o.round(u[p]);
           o.store(static_cast<T*>(a.branch_grad) + base + at[p]);
         }
