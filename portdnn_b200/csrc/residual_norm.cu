@@ -937,10 +937,12 @@ struct SumArgs {
   T* gate_grad;
 };
 
-// 32 columns to a block, sixteen threads to a column with eight loads in flight each (the matrices are in L2: bound by latency.
-// 8192x2048 bf16, eight groups, whole gradient, sixteen / 32 threads: 48.4 / 50.9 us).
-constexpr int kSumLanes = 16, kSumLoads = 8;
-template <typename T>
+// 32 columns to a block, sixteen threads to a column with LOADS loads in flight each (the matrices are in L2: bound by latency.
+// 8192x2048 bf16, eight groups, whole gradient, sixteen / 32 threads: 48.4 / 50.9 us).  Twenty loads, so that two blocks' lines to an
+// SM are one walk, where the columns are one wave of blocks, eight otherwise (whole gradients, eight / twenty: 1999x1003 f32 23.3 /
+// 21.2 us, 16384x1024 bf16 45.2 / 43.1; 640 blocks, 8192x2048 with eight groups 47.9 / 49.5; few lines, 300x4096 20.8 / 21.5).
+constexpr int kSumLanes = 16;
+template <typename T, int LOADS>
 __global__ void __launch_bounds__(32 * kSumLanes) residual_norm_sums_kernel(const SumArgs<T> a) {
   overlap_wait();
   __shared__ float red[kSumLanes][33];
@@ -951,12 +953,12 @@ __global__ void __launch_bounds__(32 * kSumLanes) residual_norm_sums_kernel(cons
   const int rows = gates ? a.parts : a.blocks, tx = (int)threadIdx.x & 31, ty = (int)threadIdx.x >> 5;
   float sum = 0.f;
   if (first + tx < n)
-    for (int r = ty; r < rows; r += kSumLanes * kSumLoads) {
-      float v[kSumLoads];
+    for (int r = ty; r < rows; r += kSumLanes * LOADS) {
+      float v[LOADS];
 #pragma unroll
-      for (int u = 0; u < kSumLoads; ++u) v[u] = r + u * kSumLanes < rows ? m[(size_t)(r + u * kSumLanes) * n + first + tx] : 0.f;
+      for (int u = 0; u < LOADS; ++u) v[u] = r + u * kSumLanes < rows ? m[(size_t)(r + u * kSumLanes) * n + first + tx] : 0.f;
 #pragma unroll
-      for (int u = 0; u < kSumLoads; ++u) sum += v[u];
+      for (int u = 0; u < LOADS; ++u) sum += v[u];
     }
   red[ty][tx] = sum;
   __syncthreads();
@@ -1308,7 +1310,10 @@ int launch_residual_norm_gradient(int dtype, const PdnnResidualNormParams& p, co
       sums.gate = static_cast<const T*>(t.gate);
       sums.gate_grad = static_cast<T*>(g.gate_grad);
       const size_t tiles = (sums.line + 31) / 32 + (sums.gate_entries + 31) / 32;
-      launch_overlapped(residual_norm_sums_kernel<T>, dim3((unsigned)tiles), 32 * kSumLanes, s, sums);
+      if (blocks > kSumLanes * 8 && tiles <= 2 * (size_t)sms)
+        launch_overlapped(residual_norm_sums_kernel<T, 20>, dim3((unsigned)tiles), 32 * kSumLanes, s, sums);
+      else
+        launch_overlapped(residual_norm_sums_kernel<T, 8>, dim3((unsigned)tiles), 32 * kSumLanes, s, sums);
       status = check_launch(what);
     }
     if (scratch != nullptr) cudaFreeAsync(scratch, s);
