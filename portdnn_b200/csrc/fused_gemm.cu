@@ -1033,11 +1033,13 @@ struct Plan {
   bool swapped;
 };
 
-// Estimated times of the plans in us, from what they measured over 24 shapes of 1 to 8192 rows (a step is 64 elements of K).
-// A pair's step takes 0.34 us at 256 columns and 0.23 at 128 (an SM pulls its 24 KB of operands through L2 no faster), two
-// thirds of that with few clusters in flight (but for fp32, whose products bound it: 2000x777x300 28.7 us, single CTAs 23.1), behind 5.5 and 4.7 us of launch, ramp and end.  A CTA alone takes 0.2 to 0.29 us a step
-// by its columns, half as much again where two share an SM, behind 3 us, 0.017 a column for its end and 0.45 for each
-// partial tile that it adds.
+// Estimated times of the plans in us, their constants fitted to all plans' times of 128 products of 1 to 8192 rows (a step is 64 elements
+// of K): over these the plan picked takes 1 % more than the best one (a fit to 24 products took 5 % more).
+// A pair's step takes 0.39 us at 256 columns and 0.29 at 128 (an SM pulls its operands through L2 no faster), three quarters of that with
+// few clusters in flight (but for fp32, whose products bound it: 2000x777x300 28.7 us, single CTAs 23.1), a tile no less than its end, 2.3
+// and 2.2 us, all behind 8.3 and 5 us of launch, ramp and the last end.  A CTA alone takes 0.21 to 0.31 us a step by its columns, two
+// thirds more where two share an SM (clusters of four and eight do before there is a CTA to every SM), behind 3.8 us, 0.022 a column for its
+// end, 0.26 for each partial tile that it adds (0.75 where it ends on its own), and 0.0018 for every CTA's reads beside it.
 Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_major, int kblocks, int sms) {
   const double products = split ? kProducts : 1;
   auto tiles = [](long long x, int t) { return (x + t - 1) / t; };
@@ -1047,8 +1049,8 @@ Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_majo
     if (split && bn == 256) continue;
     const long long all = tiles(m, 256) * tiles(n, bn);
     const double waves = (double)tiles(all, sms / 2), busy = std::min(1.0, (double)all / (sms / 2));
-    const double step = (bn == 256 ? 0.34 : 0.23) * (split ? 1.0 : 0.6 + 0.4 * busy);
-    const double t = waves * kblocks * step * products + (bn == 256 ? 5.5 : 4.7) + (split ? 2.0 : 0.0);
+    const double step = split ? 0.23 * products : (bn == 256 ? 0.39 : 0.29) * (0.77 + 0.23 * busy);
+    const double t = waves * std::max(kblocks * step, bn == 256 ? 2.28 : 2.17) + (split ? 6.7 : bn == 256 ? 8.25 : 4.98);
     if (t < least) least = t, best = Plan{true, bn, 1, false};
   }
   for (int swapped = 0; swapped < 2; ++swapped)
@@ -1062,9 +1064,9 @@ Plan choose_plan(bool split, long long m, long long n, bool m_major, bool n_majo
         const int steps = (kblocks + splits - 1) / splits;
         if (splits > 1 && steps * (splits - 1) >= kblocks) continue;  // a CTA without steps
         const long long ctas = all * splits;
-        const double waves = (double)tiles(ctas, 2ll * sms), shared = ctas > sms ? 1.5 : 1.0;
-        const double step = (bn == 128 ? 0.29 : bn == 64 ? 0.23 : 0.2) * shared;
-        const double t = 1.5 + waves * (steps * step * products + 1.5 + 0.017 * bn * shared + (splits > 1 ? 0.45 * splits : 0.0));
+        const double waves = (double)tiles(ctas, 2ll * sms), shared = ctas > sms - (splits == 8 ? 28 : splits == 4 ? 4 : 0) ? 1.65 : 1.0;
+        const double step = (bn == 128 ? 0.31 : bn == 64 ? 0.21 : 0.24) * shared;
+        const double t = 2.28 + 0.0018 * ctas + waves * (steps * step * products + 1.51 + 0.022 * bn * shared + (splits > 1 ? 0.26 * splits : 0.75));
         if (t < least) least = t, best = Plan{false, bn, splits, swapped != 0};
       }
     }
@@ -1191,7 +1193,13 @@ int run_plan(const Plan& plan, int dtype, int out_dtype, Side x, Side y, int k, 
   a.pre_vec = packets_ok(out_dtype, f.pre, f.pre_pitch);
   a.bias_vec = packets_ok(out_dtype, f.bias, 0);
   const int stage = (SPLIT ? 3 : 1) * (128 + plan.bn) * kStepK * 2;
-  a.stages = std::min(kMostStages, (kSoloSmem - kSoloHead) / stage);
+  // All of an SM's shared memory for stages where there is one CTA to an SM, with steps enough to use them (fewer where half of it holds
+  // three stages alone), and clusters small enough to be placed all the same (us, half / all: 128x4096x4096 bf16, 64 columns, 32 steps, 13.9 /
+  // 11.8; 256x2048x1000 f32 24.9 / 22.0; too few steps, 1024x1024x1024 bf16 7.7 / 8.3; clusters of eight, 130x8192x200 7.6 / 12.9).
+  const long long ctas = (long long)a.tiles_m * a.tiles_n * plan.splits;
+  const int half = (kSoloSmem - kSoloHead) / stage;
+  const bool deep = a.blocks_per_split >= (half < 4 ? 16 : 24) && ctas <= (plan.splits <= 2 ? sms : plan.splits == 4 ? 128 : 0);
+  a.stages = std::min(kMostStages, deep ? (kSmemBudget - kSoloHead) / stage : half);
   const size_t partial = plan.swapped ? (size_t)plan.bn * (128 * 4 + 16) : (size_t)128 * (plan.bn * 4 + 16);
   const size_t smem = kSoloHead + std::max((size_t)a.stages * stage, partial);
   tc_set_last_kernel("solo_gemm_kernel");
