@@ -35,7 +35,8 @@ constexpr int kChainSteps = 2;     // fp32: stages whose products the accumulato
 constexpr int kMostStages = 12;
 constexpr int kSlotBytes = 4096;   // 32 rows of 128 bytes, swizzled as TMA does
 constexpr int kSmemBudget = 232448;
-constexpr int kFewRows = 16;       // fp32 rows that go to fused_rows.cu
+// fp32 rows that go to fused_rows.cu, by the side on which the weights' rows lie
+constexpr int few_rows(bool k_rows) { return k_rows ? 16 : 24; }
 constexpr int kProducts = 6;       // products of parts that make an fp32 product
 
 struct alignas(64) FusedArgs {
@@ -1218,9 +1219,9 @@ int fused_gemm(int dtype, int ta, int tb, const Matrix& a, const Matrix& b, int 
   Plan plan = choose_plan(dtype == PDNN_F32, f.rows, f.cols, x.mn_major != 0, y.mn_major != 0, kblocks, sms);
   if (dtype == PDNN_F16) return run_plan<__half, false>(plan, dtype, dtype, x, y, k, 0, f, beside, s);
   if (dtype == PDNN_BF16) return run_plan<__nv_bfloat16, false>(plan, dtype, dtype, x, y, k, 0, f, beside, s);
-  // fp32.  Few rows: cutting the weights into parts costs more than multiplying them (4096 x 4096, us, parts / rows: 1 row 59 / 15, 16
-  // rows 59 / 47, 32 rows 60 / 78).
-  if (!ta && f.rows <= kFewRows) return fused_rows(tb != 0, a, b, k, f, s);
+  // fp32.  Few rows: cutting the weights into parts costs more than multiplying them (us, parts / rows, weights [n][k]: 4096x4096, 1 row 59 /
+  // 15, 16 rows 60 / 48, 24 rows 61 / 85; 256x7296, 16 rows 13.8 / 13.4; [k][n]: 4096x4096, 24 rows 60 / 43, 32 rows 60 / 77).
+  if (!ta && f.rows <= few_rows(tb != 0)) return fused_rows(tb != 0, a, b, k, f, s);
   // parts behind one another along K
   const int part_k = kblocks * 64;
   if (3ll * part_k > 0x7FFF0000ll) return fail(PDNN_INDEX_EXCEEDED, "matmul_fused: an fp32 sum of %d products is too long", k);  // (TMA counts in 32 bits)

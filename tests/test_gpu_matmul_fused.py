@@ -66,6 +66,23 @@ def test_forward(m, k, n, dtype, tr):
     _forward(m, k, n, tr, dtype, "gelu", True, True, 0.5, True)
 
 
+# on both sides of the numbers of rows from which fp32 products leave the CUDA cores
+@pytest.mark.parametrize("tr", [False, True])
+@pytest.mark.parametrize("m", [15, 16, 17, 23, 24, 25])
+def test_few_rows_in_single_precision(m, tr):
+    _forward(m, 300, 203, tr, "f32", "tanh", True, True, 0.7, True)
+    _forward(m, 1024, 512, tr, "f32", "none", False, False, 1.0, False)
+    _gradients(m, 300, 203, tr, "f32", "silu", "none", 1.0)
+
+
+# few tiles and long sums: clusters of every size, rings of stages that take all of an SM's shared memory or half
+@pytest.mark.parametrize("m,k,n", [(128, 4096, 2048), (256, 2048, 1000), (60, 6000, 1000), (100, 8000, 104), (700, 4160, 64), (1, 8192, 72)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tr", [False, True])
+def test_long_sums(m, k, n, dtype, tr):
+    _forward(m, k, n, tr, dtype, "silu", True, False, 1.0, True)
+
+
 @pytest.mark.parametrize("activation", sorted(ACTS))
 @pytest.mark.parametrize("m", [5, 300, 2500])
 def test_activations(activation, m):
